@@ -7,6 +7,7 @@
 #include <dlfcn.h>
 #include <nccl.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -73,6 +74,8 @@ struct g4s_ctx {
     // LM head workspace (first g4s_lmhead_sample call): fp32 logits and fp16 hidden
     float *lm_logits = nullptr;
     void *lm_xh = nullptr;
+    int4 *pg_copies = nullptr;  // [max_rows] page copies a g4s_pages_fork lists, and their count
+    int *pg_n_copies = nullptr;
     int *dev_err = nullptr;  // device error flag in the workspace (a bounded wait that ran out), read by g4s_device_status
     int64_t wait_limit = 0;  // g4s_set_wait_limit (test hook; 0 = the kernels' own limits)
     size_t lm_logits_n = 0, lm_xh_n = 0;
@@ -513,6 +516,8 @@ int32_t g4s_create(int32_t device, int32_t max_rows, int32_t max_vocab, uint32_t
     const size_t o_tab = off; off = align(off + (size_t)SC_TABLE_BYTES);
     const size_t o_etab = off; off = align(off + (size_t)ETAB_TABLE_BYTES);
     const size_t o_stg = off; off = align(off + (size_t)max_rows * sizeof(ShardTarget));
+    const size_t o_pgc = off; off = align(off + (size_t)max_rows * sizeof(int4));
+    const size_t o_pgn = off; off = align(off + sizeof(int));
     ctx->ws_bytes = off;
     if (cudaMalloc(&ctx->ws, off) != cudaSuccess) {
         cudaGetLastError();
@@ -532,6 +537,8 @@ int32_t g4s_create(int32_t device, int32_t max_rows, int32_t max_vocab, uint32_t
     ctx->sc_tab = (float *)(base + o_tab);
     ctx->e_tab = (float *)(base + o_etab);
     ctx->shard_tgt = (ShardTarget *)(base + o_stg);
+    ctx->pg_copies = (int4 *)(base + o_pgc);
+    ctx->pg_n_copies = (int *)(base + o_pgn);
     if (cudaMemset(ctx->ws, 0, off) != cudaSuccess ||
         cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking) != cudaSuccess ||
         cudaHostAlloc((void **)&ctx->params_pinned, (size_t)PSLOTS * max_rows * (sizeof(g4s_params) + sizeof(float) + sizeof(int32_t)),
@@ -1351,6 +1358,359 @@ int32_t g4s_shard_abort(g4s_ctx *ctx)
     DeviceGuard guard(ctx->device);
     if (!guard.ok) return fail(ctx, G4S_ERR_CUDA, "g4s_shard_abort: cannot select device %d", ctx->device);
     shard_release(ctx, true);
+    return G4S_OK;
+}
+
+// ---------------------------------------------------------------------------
+// beam search
+// ---------------------------------------------------------------------------
+void g4s_beam_params_defaults(g4s_beam_params *p)
+{
+    if (!p) return;
+    memset(p, 0, sizeof(*p));
+    p->beams = p->n_out = 4;
+    p->temperature = 1.0;
+    p->n_eos = 3;
+    p->eos[0] = 1;
+    p->eos[1] = 106;
+    p->eos[2] = 50;
+}
+
+// Whether out may be written while in is read: other memory, or (same) the very same array.
+static bool aliasing_ok(const void *in, const void *out, size_t in_bytes, size_t out_bytes, bool same)
+{
+    if (!in || !out) return true;
+    if (in == out) return same;
+    const char *a = (const char *)in, *b = (const char *)out;
+    return a + in_bytes <= b || b + out_bytes <= a;
+}
+
+static int pow2_at_least(int n)
+{
+    int p = 2;
+    while (p < n) p <<= 1;
+    return p;
+}
+
+static int32_t beam_select_args(g4s_ctx *ctx, const char *who, const void *logits, int32_t dtype, int32_t groups,
+                                int32_t vocab, int64_t row_stride, float softcap, const g4s_beam_params *p,
+                                const g4s_beam_state *in, const g4s_beam_state *out, int32_t *out_parents,
+                                int32_t *out_tokens, BeamArgs &a, bool &vec)
+{
+    if (!logits || !p || !in || !out || !out_parents || !out_tokens || !in->scores || !out->scores)
+        return fail(ctx, G4S_ERR_ARG,
+                    "%s: logits, params, in, out, their scores, out_parents and out_tokens must be non-NULL", who);
+    if (dtype != G4S_F32 && dtype != G4S_BF16) return fail(ctx, G4S_ERR_ARG, "%s: bad dtype %d", who, dtype);
+    if (p->beams < 1 || p->beams > G4S_BEAM_MAX || p->n_out < 1 || p->n_out > G4S_BEAM_MAX_OUT)
+        return fail(ctx, G4S_ERR_ARG, "%s: beams %d outside [1, %d] or n_out %d outside [1, %d]", who, p->beams,
+                    G4S_BEAM_MAX, p->n_out, G4S_BEAM_MAX_OUT);
+    if (groups < 1 || vocab < 1)
+        return fail(ctx, G4S_ERR_ARG, "%s: groups (%d) and vocab (%d) must be >= 1", who, groups, vocab);
+    if ((int64_t)groups * p->beams > ctx->max_rows || vocab > ctx->max_vocab)
+        return fail(ctx, G4S_ERR_CAPACITY, "%s: %d groups of %d beams / vocab %d exceed the context (%d / %d)", who,
+                    groups, p->beams, vocab, ctx->max_rows, ctx->max_vocab);
+    if (row_stride < vocab)
+        return fail(ctx, G4S_ERR_ARG, "%s: row_stride %lld < vocab %d", who, (long long)row_stride, vocab);
+    const size_t esize = dtype == G4S_F32 ? 4u : 2u;
+    if ((uintptr_t)logits % esize) return fail(ctx, G4S_ERR_ARG, "%s: logits are not aligned to their type", who);
+    if (!(p->temperature >= 1e-6 && p->temperature <= 1e6))
+        return fail(ctx, G4S_ERR_ARG, "%s: temperature %g outside [1e-6, 1e6]", who, p->temperature);
+    if (!(p->length_alpha >= 0.0 && p->length_alpha <= 8.0))
+        return fail(ctx, G4S_ERR_ARG, "%s: length_alpha %g outside [0, 8]", who, p->length_alpha);
+    if (!(softcap <= 0.0f || (softcap >= 1e-6f && softcap <= 1e6f)))
+        return fail(ctx, G4S_ERR_ARG, "%s: softcap %g is neither <= 0 nor within [1e-6, 1e6]", who, softcap);
+    if (p->n_eos < 0 || p->n_eos > G4S_BEAM_MAX_EOS)
+        return fail(ctx, G4S_ERR_ARG, "%s: n_eos %d outside [0, %d]", who, p->n_eos, G4S_BEAM_MAX_EOS);
+    if (!in->lens && (p->length_alpha != 0.0 || out->lens))
+        return fail(ctx, G4S_ERR_ARG, "%s: in->lens is NULL with a length_alpha or out->lens", who);
+    const size_t ni = (size_t)groups * p->beams, no = (size_t)groups * p->n_out;
+    const bool same = p->n_out == p->beams;
+    if (!aliasing_ok(in->scores, out->scores, ni * 4, no * 4, same) ||
+        !aliasing_ok(in->lens, out->lens, ni * 4, no * 4, same) || !aliasing_ok(in->done, out->done, ni, no, same))
+        return fail(ctx, G4S_ERR_ARG, "%s: out overlaps in (allowed: the same arrays, with n_out == beams)", who);
+
+    memset(&a, 0, sizeof(a));
+    a.logits = logits;
+    a.row_stride = row_stride;
+    a.rows = groups * p->beams;
+    a.beams = p->beams;
+    a.vocab = vocab;
+    a.n_out = p->n_out;
+    const int unit = beam_unit_logits(dtype), units = (int)ceil_div(vocab, unit);
+    a.upi = (int)ceil_div(units, BEAM_MAX_ITEMS);
+    a.ipr = (int)ceil_div(units, a.upi);
+    a.pe = pow2_at_least(p->beams * p->n_out);
+    a.pc = pow2_at_least(p->n_out * (p->n_out + 1) / 2);
+    a.softcap = softcap > 0.0f ? softcap : 0.0f;
+    a.invcap = softcap > 0.0f ? 1.0f / softcap : 0.0f;
+    a.k64 = 1.4426950408889634074 / p->temperature;
+    a.k = (float)a.k64;
+    a.temperature = p->temperature;
+    a.alpha = p->length_alpha;
+    a.pad_token = p->pad_token;
+    a.n_eos = p->n_eos;
+    memcpy(a.eos, p->eos, sizeof(a.eos));
+    a.scores = in->scores;
+    a.lens = in->lens;
+    a.done = in->done;
+    a.out_scores = out->scores;
+    a.out_lens = out->lens;
+    a.out_done = out->done;
+    a.out_parents = out_parents;
+    a.out_tokens = out_tokens;
+    a.istat = ctx->istat;
+    vec = ((uintptr_t)logits % 16u == 0) && ((row_stride * (int64_t)esize) % 16 == 0);
+    return G4S_OK;
+}
+
+// Largest of 16, 4 and 1 that divides every value of `bits` (addresses and sizes or-ed together).
+static int copy_width(uint64_t bits) { return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1; }
+
+static int32_t beam_reorder_args(g4s_ctx *ctx, const char *who, const int32_t *parents, int32_t groups, int32_t beams,
+                                 const g4s_beam_tensor *tensors, int32_t n_tensors, ReorderArgs &a, int64_t &blocks)
+{
+    if (n_tensors < 0 || n_tensors > G4S_BEAM_MAX_TENSORS)
+        return fail(ctx, G4S_ERR_ARG, "%s: n_tensors %d outside [0, %d]", who, n_tensors, G4S_BEAM_MAX_TENSORS);
+    if (!parents || (n_tensors && !tensors)) return fail(ctx, G4S_ERR_ARG, "%s: parents or tensors is NULL", who);
+    if (beams < 1 || beams > G4S_BEAM_MAX || groups < 1 || (int64_t)groups * beams > 0x7fffffff - G4S_BEAM_MAX)
+        return fail(ctx, G4S_ERR_ARG, "%s: beams %d outside [1, %d], or %d groups", who, beams, G4S_BEAM_MAX, groups);
+    a.parents = parents;
+    a.beams = beams;
+    a.n = 0;
+    blocks = 0;
+    for (int i = 0; i < n_tensors; i++) {
+        const g4s_beam_tensor &t = tensors[i];
+        if (t.segs0 < 1 || t.segs1 < 1 || t.seg_bytes < 0 || t.row_stride < 0 || t.stride0 < 0 || t.stride1 < 0)
+            return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d]: a negative stride or size, or no segment", who, i);
+        if (t.seg_bytes == 0) continue;
+        if (!t.src || !t.dst) return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d]: NULL src or dst", who, i);
+        if (groups * (int64_t)beams > 1 && t.row_stride < t.seg_bytes)
+            return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d]: row_stride %lld < seg_bytes %lld", who, i,
+                        (long long)t.row_stride, (long long)t.seg_bytes);
+        if ((t.segs0 > 1 && t.stride0 < t.seg_bytes) || (t.segs1 > 1 && t.stride1 < t.seg_bytes))
+            return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d]: segments overlap", who, i);
+        ReorderTensor &q = a.t[a.n];
+        q.width = copy_width((uint64_t)(uintptr_t)t.src | (uint64_t)(uintptr_t)t.dst | (uint64_t)t.seg_bytes |
+                             (uint64_t)t.row_stride | (t.segs0 > 1 ? (uint64_t)t.stride0 : 0) |
+                             (t.segs1 > 1 ? (uint64_t)t.stride1 : 0));
+        const int64_t seg_cols = t.seg_bytes / q.width, segs = (int64_t)t.segs0 * t.segs1;
+        if (seg_cols > 0x7fffffff || segs > 0x7fffffff || segs * seg_cols > 0x7fffffff)
+            return fail(ctx, G4S_ERR_CAPACITY, "%s: tensors[%d]: over 2^31 columns of %d bytes a row", who, i, q.width);
+        q.src = (const char *)t.src;
+        q.dst = (char *)t.dst;
+        q.row_stride = t.row_stride;
+        q.stride0 = t.stride0;
+        q.stride1 = t.stride1;
+        q.segs1 = (uint32_t)t.segs1;
+        q.seg_cols = (uint32_t)seg_cols;
+        q.cols = (uint32_t)(segs * seg_cols);
+        q.blocks = (uint32_t)ceil_div(q.cols, REORDER_THREADS);
+        a.first[a.n++] = blocks;
+        blocks += (int64_t)groups * q.blocks;
+        if (blocks > 0x7fffffff) return fail(ctx, G4S_ERR_CAPACITY, "%s: over 2^31 blocks of work", who);
+    }
+    return G4S_OK;
+}
+
+static int32_t pages_cache_args(g4s_ctx *ctx, const char *who, const g4s_page_cache *c, PagesArgs &a, PoolArgs &pools)
+{
+    if (!c) return fail(ctx, G4S_ERR_ARG, "%s: cache is NULL", who);
+    if (c->page_tokens < 1 || c->n_pages < 1 || c->max_seq_pages < 1 ||
+        (int64_t)c->max_seq_pages * c->page_tokens > 0x3fffffff || c->n_pages > 0x3fffffff)
+        return fail(ctx, G4S_ERR_ARG,
+                    "%s: page_tokens %d, n_pages %d and max_seq_pages %d must be >= 1, pages and a sequence's positions "
+                    "below 2^30",
+                    who, c->page_tokens, c->n_pages, c->max_seq_pages);
+    if (c->n_pools < 0 || c->n_pools > G4S_PAGES_MAX_POOLS || (c->n_pools && !c->pools))
+        return fail(ctx, G4S_ERR_ARG, "%s: n_pools %d outside [0, %d], or pools is NULL", who, c->n_pools,
+                    G4S_PAGES_MAX_POOLS);
+    memset(&a, 0, sizeof(a));
+    a.page_tokens = c->page_tokens;
+    a.n_pages = c->n_pages;
+    a.width = c->max_seq_pages;
+    pools.n = c->n_pools;
+    pools.chunks = 1;
+    for (int i = 0; i < c->n_pools; i++) {
+        const g4s_page_pool &p = c->pools[i];
+        if (!p.data || p.segs < 1 || p.token_bytes < 1 || p.page_stride < 1 || p.seg_stride < 0)
+            return fail(ctx, G4S_ERR_ARG, "%s: pools[%d]: NULL data, or a size below 1", who, i);
+        PoolArg &q = pools.p[i];
+        q.width = copy_width((uint64_t)(uintptr_t)p.data | (uint64_t)p.page_stride | (uint64_t)p.token_bytes |
+                             (p.segs > 1 ? (uint64_t)p.seg_stride : 0));
+        const int64_t vecs = p.token_bytes / q.width;
+        if (vecs > 0x7fffffff || vecs * c->page_tokens > 0x7fffffff || vecs * c->page_tokens * p.segs > 0x7fffffff)
+            return fail(ctx, G4S_ERR_CAPACITY, "%s: pools[%d]: a page of over 2^31 vectors of %d bytes", who, i, q.width);
+        const int64_t seg = p.token_bytes * c->page_tokens;
+        if ((p.segs > 1 && p.seg_stride < seg) || p.page_stride < seg + (int64_t)(p.segs - 1) * (p.segs > 1 ? p.seg_stride : 0))
+            return fail(ctx, G4S_ERR_ARG, "%s: pools[%d]: segments or pages overlap", who, i);
+        q.data = (char *)p.data;
+        q.page_stride = p.page_stride;
+        q.seg_stride = p.seg_stride;
+        q.segs = p.segs;
+        q.token_vecs = (uint32_t)vecs;
+        pools.chunks = std::max<int>(pools.chunks, (int)ceil_div(vecs * c->page_tokens * p.segs, pages_chunk_vecs()));
+    }
+    return G4S_OK;
+}
+
+static int32_t pages_seqs_ok(g4s_ctx *ctx, const char *who, int32_t n, const char *what)
+{
+    const int most = std::min(ctx->max_rows, G4S_PAGES_MAX_SEQS);
+    if (n < 0) return fail(ctx, G4S_ERR_ARG, "%s: %s %d < 0", who, what, n);
+    if (n > most) return fail(ctx, G4S_ERR_CAPACITY, "%s: %s %d above %d", who, what, n, most);
+    return G4S_OK;
+}
+
+static int32_t pages_fork_args(g4s_ctx *ctx, const char *who, const g4s_page_cache *cache, int32_t n_in,
+                               const g4s_page_tables *in, int32_t n_out, const int32_t *src, int32_t n_new,
+                               const uint8_t *frozen, const g4s_page_tables *out, int32_t *result, PagesArgs &a,
+                               PoolArgs &pools)
+{
+    int32_t rc = pages_cache_args(ctx, who, cache, a, pools);
+    if (rc != G4S_OK) return rc;
+    if ((rc = pages_seqs_ok(ctx, who, n_in, "n_in")) != G4S_OK || (rc = pages_seqs_ok(ctx, who, n_out, "n_out")) != G4S_OK)
+        return rc;
+    if (!in || !out || !result || !in->refs || !out->refs || (n_in && (!in->tables || !in->lens)) ||
+        (n_out && (!out->tables || !out->lens || !src)))
+        return fail(ctx, G4S_ERR_ARG, "%s: in, out, their arrays, src and result must be non-NULL", who);
+    if (n_new < 0 || n_new > 0x3fffffff) return fail(ctx, G4S_ERR_ARG, "%s: n_new %d outside [0, 2^30)", who, n_new);
+    const size_t wi = (size_t)n_in * a.width * 4, wo = (size_t)n_out * a.width * 4, np = (size_t)a.n_pages * 4;
+    if (n_in && n_out && !aliasing_ok(in->tables, out->tables, wi, wo, false))
+        return fail(ctx, G4S_ERR_ARG, "%s: out->tables overlaps in->tables", who);
+    if (!aliasing_ok(in->refs, out->refs, np, np, true) ||
+        (n_in && n_out && !aliasing_ok(in->lens, out->lens, (size_t)n_in * 4, (size_t)n_out * 4, true)))
+        return fail(ctx, G4S_ERR_ARG, "%s: out's refs or lens overlap in's (allowed: the same arrays)", who);
+    a.n_in = n_in;
+    a.n_out = n_out;
+    a.n_new = n_new;
+    a.max_copies = n_out;
+    a.tables_in = in->tables;
+    a.lens_in = in->lens;
+    a.refs_in = in->refs;
+    a.src = src;
+    a.frozen = frozen;
+    a.tables_out = out->tables;
+    a.lens_out = out->lens;
+    a.refs_out = out->refs;
+    a.result = result;
+    a.copies = ctx->pg_copies;
+    a.n_copies = ctx->pg_n_copies;
+    return G4S_OK;
+}
+
+int32_t g4s_beam_select(g4s_ctx *ctx, const void *logits, int32_t dtype, int32_t groups, int32_t vocab,
+                        int64_t row_stride, float softcap, const g4s_beam_params *params, const g4s_beam_state *in,
+                        const g4s_beam_state *out, int32_t *out_parents, int32_t *out_tokens, void *stream)
+{
+    static const char *who = "g4s_beam_select";
+    if (!ctx) return fail(nullptr, G4S_ERR_ARG, "%s: ctx is NULL", who);
+    BeamArgs a;
+    bool vec;
+    const int32_t rc = beam_select_args(ctx, who, logits, dtype, groups, vocab, row_stride, softcap, params, in, out,
+                                        out_parents, out_tokens, a, vec);
+    if (rc != G4S_OK) return rc;
+    DeviceGuard guard(ctx->device);
+    if (!guard.ok) return fail(ctx, G4S_ERR_CUDA, "%s: cannot select device %d", who, ctx->device);
+    const cudaError_t e = launch_beam_select(a, dtype, vec, ctx->sm_count, stream ? (cudaStream_t)stream : ctx->stream);
+    if (e != cudaSuccess) return fail(ctx, G4S_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
+    return G4S_OK;
+}
+
+int32_t g4s_beam_reorder(g4s_ctx *ctx, const int32_t *parents, int32_t groups, int32_t beams,
+                         const g4s_beam_tensor *tensors, int32_t n_tensors, void *stream)
+{
+    static const char *who = "g4s_beam_reorder";
+    if (!ctx) return fail(nullptr, G4S_ERR_ARG, "%s: ctx is NULL", who);
+    ReorderArgs a;
+    int64_t blocks = 0;
+    const int32_t rc = beam_reorder_args(ctx, who, parents, groups, beams, tensors, n_tensors, a, blocks);
+    if (rc != G4S_OK || blocks == 0) return rc;
+    DeviceGuard guard(ctx->device);
+    if (!guard.ok) return fail(ctx, G4S_ERR_CUDA, "%s: cannot select device %d", who, ctx->device);
+    const cudaError_t e = launch_beam_reorder(a, blocks, stream ? (cudaStream_t)stream : ctx->stream);
+    if (e != cudaSuccess) return fail(ctx, G4S_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
+    return G4S_OK;
+}
+
+int32_t g4s_pages_fork(g4s_ctx *ctx, const g4s_page_cache *cache, int32_t n_in, const g4s_page_tables *in,
+                       int32_t n_out, const int32_t *src, int32_t n_new, const uint8_t *frozen,
+                       const g4s_page_tables *out, int32_t *result, void *stream)
+{
+    static const char *who = "g4s_pages_fork";
+    if (!ctx) return fail(nullptr, G4S_ERR_ARG, "%s: ctx is NULL", who);
+    PagesArgs a;
+    PoolArgs pools;
+    const int32_t rc = pages_fork_args(ctx, who, cache, n_in, in, n_out, src, n_new, frozen, out, result, a, pools);
+    if (rc != G4S_OK) return rc;
+    DeviceGuard guard(ctx->device);
+    if (!guard.ok) return fail(ctx, G4S_ERR_CUDA, "%s: cannot select device %d", who, ctx->device);
+    const cudaError_t e = launch_pages_fork(a, pools, ctx->sm_count, stream ? (cudaStream_t)stream : ctx->stream);
+    if (e != cudaSuccess) return fail(ctx, G4S_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
+    return G4S_OK;
+}
+
+int32_t g4s_pages_compact(g4s_ctx *ctx, const g4s_page_cache *cache, int32_t n_seqs, const g4s_page_tables *in,
+                          const g4s_page_tables *out, int32_t *page_map, int32_t *moves, int32_t *result, void *stream)
+{
+    static const char *who = "g4s_pages_compact";
+    if (!ctx) return fail(nullptr, G4S_ERR_ARG, "%s: ctx is NULL", who);
+    PagesArgs a;
+    PoolArgs pools;
+    int32_t rc = pages_cache_args(ctx, who, cache, a, pools);
+    if (rc != G4S_OK || (rc = pages_seqs_ok(ctx, who, n_seqs, "n_seqs")) != G4S_OK) return rc;
+    if (!in || !out || !page_map || !moves || !result || !in->refs || !out->refs ||
+        (n_seqs && (!in->tables || !in->lens || !out->tables)))
+        return fail(ctx, G4S_ERR_ARG, "%s: in, out, their arrays, page_map, moves and result must be non-NULL", who);
+    const size_t w = (size_t)n_seqs * a.width * 4, np = (size_t)a.n_pages * 4;
+    if ((n_seqs && !aliasing_ok(in->tables, out->tables, w, w, true)) || !aliasing_ok(in->refs, out->refs, np, np, true))
+        return fail(ctx, G4S_ERR_ARG, "%s: out's tables or refs overlap in's (allowed: the same arrays)", who);
+    a.n_in = a.n_out = n_seqs;
+    a.max_copies = a.n_pages / 2;
+    a.tables_in = in->tables;
+    a.lens_in = in->lens;
+    a.refs_in = in->refs;
+    a.tables_out = out->tables;
+    a.refs_out = out->refs;
+    a.page_map = page_map;
+    a.moves = moves;
+    a.result = result;
+    DeviceGuard guard(ctx->device);
+    if (!guard.ok) return fail(ctx, G4S_ERR_CUDA, "%s: cannot select device %d", who, ctx->device);
+    const cudaError_t e = launch_pages_compact(a, pools, ctx->sm_count, stream ? (cudaStream_t)stream : ctx->stream);
+    if (e != cudaSuccess) return fail(ctx, G4S_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
+    return G4S_OK;
+}
+
+int32_t g4s_beam_step(g4s_ctx *ctx, const void *logits, int32_t dtype, int32_t groups, int32_t vocab,
+                      int64_t row_stride, float softcap, const g4s_beam_params *params, const g4s_beam_state *in,
+                      const g4s_beam_state *out, int32_t *out_parents, int32_t *out_tokens,
+                      const g4s_beam_tensor *tensors, int32_t n_tensors, const g4s_beam_pages *pages, void *stream)
+{
+    static const char *who = "g4s_beam_step";
+    if (!ctx) return fail(nullptr, G4S_ERR_ARG, "%s: ctx is NULL", who);
+    BeamArgs a;
+    bool vec;
+    int32_t rc = beam_select_args(ctx, who, logits, dtype, groups, vocab, row_stride, softcap, params, in, out,
+                                  out_parents, out_tokens, a, vec);
+    if (rc != G4S_OK) return rc;
+    if (params->n_out != params->beams)
+        return fail(ctx, G4S_ERR_ARG, "%s: n_out %d is not beams %d", who, params->n_out, params->beams);
+    ReorderArgs r;
+    int64_t blocks = 0;
+    if ((rc = beam_reorder_args(ctx, who, out_parents, groups, params->beams, tensors, n_tensors, r, blocks)) != G4S_OK)
+        return rc;
+    PagesArgs p;
+    PoolArgs pools;
+    if (pages && (rc = pages_fork_args(ctx, who, pages->cache, a.rows, &pages->in, a.rows, out_parents, pages->n_new,
+                                       out->done, &pages->out, pages->result, p, pools)) != G4S_OK)
+        return rc;
+    DeviceGuard guard(ctx->device);
+    if (!guard.ok) return fail(ctx, G4S_ERR_CUDA, "%s: cannot select device %d", who, ctx->device);
+    cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+    cudaError_t e = launch_beam_select(a, dtype, vec, ctx->sm_count, s);
+    if (e == cudaSuccess && blocks) e = launch_beam_reorder(r, blocks, s);
+    if (e == cudaSuccess && pages) e = launch_pages_fork(p, pools, ctx->sm_count, s);
+    if (e != cudaSuccess) return fail(ctx, G4S_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     return G4S_OK;
 }
 

@@ -118,56 +118,12 @@ __device__ __forceinline__ void s_of_many(const float *x, const SParams &sp, flo
     }
 }
 
-__device__ __forceinline__ float fmax_nan(float a, float b)
-{
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float fmin_nan(float a, float b)
-{
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float fmax3_nan(float a, float b, float c)
-{
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-__device__ __forceinline__ float fmin3_nan(float a, float b, float c)
-{
-    float r;
-    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-__device__ __forceinline__ uint32_t bmax2_nan(uint32_t a, uint32_t b)
-{
-    uint32_t r;
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t bmin2_nan(uint32_t a, uint32_t b)
-{
-    uint32_t r;
-    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 __device__ __forceinline__ float warp_max_nan(float v)
 {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v = fmax_nan(v, __shfl_xor_sync(FULLMASK, v, d));
     return v;
 }
-// Warp maximum of non-NaN floats in one instruction (sm_100a).
-__device__ __forceinline__ float warp_max_redux(float v)
-{
-    float r;
-    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
-}
-
 // Item `sub` of a row holds n = min(ITEM, vocab - sub * ITEM) logits.
 template <int DT>
 __device__ __forceinline__ int item_len(int vocab, int sub)

@@ -212,4 +212,75 @@ cudaError_t launch_etable(float cap, float invcap, float invT, bool use_t, float
 // Whether a call's full-path rows may take the E-table kernel, and its grid size per SM.
 int full_etab_blocks_per_sm();
 
+
+// ---------------------------------------------------------------------------
+// beam search (g4s_beam.cu, g4s_pages.cu)
+// ---------------------------------------------------------------------------
+constexpr int BEAM_MAX_ITEMS = 512;  // items a row in the selection's statistics
+constexpr int BEAM_COMBINE_SMEM_MAX = (2048 + 4096) * 16;  // 32 beams, 64 continuations
+
+struct BeamArgs {
+    const void *logits;
+    int64_t row_stride;   // elements
+    int rows, beams, vocab, n_out;
+    int upi, ipr;         // 2 KiB units an item, items a row
+    int pe, pc;           // combine: sort sizes (powers of two) of the items and of the tokens
+    float softcap, invcap, k;  // k = log2(e) / temperature
+    double k64, temperature, alpha;
+    int pad_token, n_eos, eos[G4S_BEAM_MAX_EOS];
+    const float *scores;
+    const int32_t *lens;
+    const uint8_t *done;
+    float *out_scores;
+    int32_t *out_lens;
+    uint8_t *out_done;
+    int32_t *out_parents, *out_tokens;
+    float4 *istat;        // [rows][ipr] (m, c, S, -)
+};
+// Logits of a 2 KiB unit.
+int beam_unit_logits(int dtype);
+cudaError_t launch_beam_select(const BeamArgs &a, int dtype, bool vec, int sms, cudaStream_t s);
+
+constexpr int REORDER_THREADS = 256;
+struct ReorderTensor {
+    const char *src;
+    char *dst;
+    int64_t row_stride, stride0, stride1;  // bytes
+    uint32_t segs1, seg_cols, cols, blocks;  // columns a segment and a row; blocks a group
+    int width;                               // bytes a column: 16, 4 or 1
+};
+struct ReorderArgs {
+    const int32_t *parents;
+    int beams, n;
+    int64_t first[G4S_BEAM_MAX_TENSORS];  // each tensor's first block
+    ReorderTensor t[G4S_BEAM_MAX_TENSORS];
+};
+cudaError_t launch_beam_reorder(const ReorderArgs &a, int64_t blocks, cudaStream_t s);
+
+struct PagesArgs {
+    int page_tokens, n_pages, width;   // width: entries of a table's row
+    int n_in, n_out, n_new, max_copies;
+    const int32_t *tables_in, *lens_in, *refs_in, *src;
+    const uint8_t *frozen;
+    int32_t *tables_out, *lens_out, *refs_out, *result;
+    int32_t *page_map, *moves;         // compaction
+    int4 *copies;                      // fork: (from, to, filled positions)
+    int *n_copies;
+};
+struct PoolArg {
+    char *data;
+    int64_t page_stride, seg_stride;   // bytes
+    int segs;
+    uint32_t token_vecs;               // vectors a position and segment
+    int width;                         // bytes a vector: 16, 4 or 1
+};
+struct PoolArgs {
+    int n, chunks;                     // chunks of pages_chunk_vecs() vectors a page
+    PoolArg p[G4S_PAGES_MAX_POOLS];
+};
+int pages_chunk_vecs();
+int pages_fork_smem(int n_in, int n_out);
+cudaError_t launch_pages_fork(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s);
+cudaError_t launch_pages_compact(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s);
+
 }  // namespace g4s

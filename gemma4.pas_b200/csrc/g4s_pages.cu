@@ -1,0 +1,418 @@
+// g4s_pages.cu -- the pages of a beam search's cache: forking by parents with
+// copy on write, allocation and freeing (pages_fork_kernel), compaction
+// (pages_compact_kernel), and the copies of page contents that both list
+// (pages_copy_kernel).  No counterpart in the reference, whose cache is one
+// contiguous ring a layer (src/Gemma4.Model.pas:61-66).
+//
+// What decides (tables, lengths, counts) is whole numbers and a few hundred
+// KiB: one thread-block cluster walks it, its barriers standing between the
+// steps, so that a fork is two launches whatever its size.  What moves bytes
+// runs over the whole GPU as the first kernel's programmatic dependent.
+#include <cooperative_groups.h>
+
+#include "g4s_device.cuh"
+#include "g4s_kernels.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace g4s {
+
+constexpr int PG_CLUSTER = 8;       // CTAs of the cluster that decides
+constexpr int PG_THREADS = 1024;
+constexpr int PG_WARPS = PG_THREADS / 32;
+constexpr int PG_SLICES = PG_CLUSTER * PG_WARPS;  // a warp's slice of the page counts
+constexpr int PC_THREADS = 256;     // CTA of the copies
+constexpr int PC_VECS = 4;          // vectors a thread and step
+
+// Exclusive scan over the CTA's PG_THREADS values; *total gets the sum.  sh: PG_WARPS + 1 ints.
+__device__ __forceinline__ int pg_scan(int v, int *total, int *sh)
+{
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int inc = warp_incl_scan(v);
+    if (lane == 31) sh[w] = inc;
+    __syncthreads();
+    if (w == 0) {
+        const int s = sh[lane];
+        const int si = warp_incl_scan(s);
+        sh[lane] = si - s;
+        if (lane == 31) sh[PG_WARPS] = si;
+    }
+    __syncthreads();
+    const int r = sh[w] + inc - v;
+    *total = sh[PG_WARPS];
+    __syncthreads();
+    return r;
+}
+
+__device__ __forceinline__ int64_t pages_of(int64_t tokens, int page_tokens)
+{
+    return (tokens + page_tokens - 1) / page_tokens;
+}
+
+// A sequence's length, or -1 where the table cannot hold it.
+__device__ __forceinline__ int seq_len(const PagesArgs &a, int i)
+{
+    const int n = a.lens_in[i];
+    return n >= 0 && (int64_t)n <= (int64_t)a.width * a.page_tokens ? n : -1;
+}
+
+// Fork.  Dynamic shared memory, n = max(n_in, n_out): children of each old sequence, and
+// of each new one its length, last page if it has to be its own, its place in the
+// allocation and in the copies.
+__global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const PagesArgs a)
+{
+    cg::cluster_group cluster = cg::this_cluster();
+    extern __shared__ int s_dyn[];
+    __shared__ int s_free[PG_WARPS], s_sh[PG_WARPS + 1], s_pref[PG_SLICES], s_bad, s_over, s_allbad;
+    const int rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int gw = rank * PG_WARPS + warp, gt = rank * PG_THREADS + tid;
+    const int P = a.page_tokens, nmax = max(a.n_in, a.n_out);
+    int *s_kids = s_dyn, *s_len = s_kids + a.n_in, *s_last = s_len + nmax, *s_off = s_last + nmax, *s_cp = s_off + nmax;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    if (tid == 0) s_bad = s_over = 0;
+    for (int i = tid; i < a.n_in; i += PG_THREADS) s_kids[i] = 0;
+    if (a.refs_out != a.refs_in)
+        for (int p = gt; p < a.n_pages; p += PG_CLUSTER * PG_THREADS) a.refs_out[p] = a.refs_in[p];
+    __syncthreads();
+    for (int j = tid; j < a.n_out; j += PG_THREADS) {
+        const int p = a.src[j];
+        int len = 0;
+        if (p >= 0) {
+            len = p < a.n_in ? seq_len(a, p) : -1;
+            if (len >= 0) atomicAdd(&s_kids[p], 1);
+            else if (rank == 0) atomicAdd(&s_bad, 1);
+        }
+        s_len[j] = p >= 0 && len >= 0 ? len : -1;  // -1: an empty sequence
+    }
+    cluster.sync();  // the counts are copied
+
+    // each old sequence's pages lose its hold and gain its children's
+    for (int i = gw; i < a.n_in; i += PG_SLICES) {
+        const int d = s_kids[i] - 1, len = seq_len(a, i);
+        if (d == 0 || len <= 0) continue;
+        const int32_t *row = a.tables_in + (int64_t)i * a.width;
+        for (int c = lane; c < pages_of(len, P); c += 32) {
+            const int p = row[c];
+            if (p >= 0 && p < a.n_pages) atomicAdd(&a.refs_out[p], d);
+        }
+    }
+    for (int j = gw; j < a.n_out; j += PG_SLICES) {
+        if (s_len[j] <= 0) continue;
+        const int32_t *row = a.tables_in + (int64_t)a.src[j] * a.width;
+        int32_t *to = a.tables_out + (int64_t)j * a.width;
+        int bad = 0;
+        for (int c = lane; c < pages_of(s_len[j], P); c += 32) {
+            const int p = row[c];
+            to[c] = p;
+            bad += p < 0 || p >= a.n_pages;
+        }
+        bad = __reduce_add_sync(FULLMASK, bad);
+        if (lane == 0 && bad) atomicAdd(&s_bad, bad);
+    }
+    cluster.sync();  // the counts are the fork's
+
+    // free pages of each warp's slice
+    const int per = (a.n_pages + PG_SLICES - 1) / PG_SLICES;
+    const int64_t lo = (int64_t)gw * per;
+    const int n_slice = (int)max((int64_t)0, min((int64_t)per, a.n_pages - lo));
+    {
+        int n = 0;
+        for (int i = lane; i < n_slice; i += 32) n += __ldcg(a.refs_out + lo + i) <= 0;
+        n = __reduce_add_sync(FULLMASK, n);
+        if (lane == 0) s_free[warp] = n;
+    }
+    // every CTA works out every sequence's needs (a page that only one holds stays its
+    // own; of w writers of a page with r holds, the first min(w, r - 1) copy it)
+    for (int j = tid; j < a.n_out; j += PG_THREADS) {
+        const int len = s_len[j];
+        int last = -1;
+        if (a.n_new > 0 && len > 0 && len % P && !(a.frozen && a.frozen[j])) {
+            last = a.tables_in[(int64_t)a.src[j] * a.width + len / P];
+            if (last < 0 || last >= a.n_pages) last = -1;
+        }
+        s_last[j] = last;
+    }
+    __syncthreads();
+    int base = 0, cbase = 0;
+    for (int j0 = 0; j0 < a.n_out; j0 += PG_THREADS) {
+        const int j = j0 + tid;
+        int need = 0, copy = 0;
+        if (j < a.n_out && s_len[j] >= 0 && a.n_new > 0 && !(a.frozen && a.frozen[j])) {
+            const int len = s_len[j], last = s_last[j];
+            if (last >= 0) {
+                const int holds = __ldcg(a.refs_out + last);
+                if (holds > 1) {
+                    int before = 0;
+                    for (int i = 0; i < j; i++) before += s_last[i] == last;
+                    copy = before < holds - 1;
+                }
+            }
+            const int64_t now = pages_of(len, P), then = pages_of((int64_t)len + a.n_new, P);
+            if (then > a.width) {
+                if (rank == 0) atomicAdd(&s_over, 1);
+            } else {
+                need = copy + (int)(then - now);
+            }
+        }
+        int total, ctotal;
+        const int off = pg_scan(need, &total, s_sh), coff = pg_scan(copy, &ctotal, s_sh);
+        if (j < a.n_out) {
+            s_off[j] = base + off;
+            s_cp[j] = copy ? cbase + coff : -1;
+        }
+        base += total;
+        cbase += ctotal;
+    }
+    cluster.sync();  // the slices' free pages, the bad entries
+
+    if (tid < PG_SLICES) s_pref[tid] = *cluster.map_shared_rank(&s_free[tid % PG_WARPS], tid / PG_WARPS);
+    if (tid == PG_SLICES) {
+        int bad = 0;
+        for (int r = 0; r < PG_CLUSTER; r++) bad += *cluster.map_shared_rank(&s_bad, r);
+        s_allbad = bad;
+    }
+    if (tid == PG_SLICES + 1 && rank) s_over = *cluster.map_shared_rank(&s_over, 0);
+    __syncthreads();
+    int free_pages;
+    const int pref = pg_scan(tid < PG_SLICES ? s_pref[tid] : 0, &free_pages, s_sh);
+    if (tid < PG_SLICES) s_pref[tid] = pref;
+    __syncthreads();
+    const bool ok = base <= free_pages && s_over == 0 && s_allbad == 0;
+    if (ok && s_pref[gw] < base) {
+        // the k-th free page belongs to the last sequence whose place is at or before k
+        int k0 = s_pref[gw];
+        for (int i0 = 0; i0 < n_slice && k0 < base; i0 += 32) {
+            const int p = (int)lo + i0 + lane;
+            const bool is = i0 + lane < n_slice && __ldcg(a.refs_out + p) <= 0;
+            const unsigned b = __ballot_sync(FULLMASK, is);
+            const int k = k0 + __popc(b & ((1u << lane) - 1));
+            k0 += __popc(b);
+            if (!is || k >= base) continue;
+            int j = 0, hi = a.n_out - 1;
+            while (j < hi) {
+                const int mid = (j + hi + 1) / 2;
+                if (s_off[mid] <= k) j = mid;
+                else hi = mid - 1;
+            }
+            const int len = s_len[j], t = k - s_off[j], slot = s_cp[j];
+            a.refs_out[p] = 1;
+            if (slot >= 0 && t == 0) {
+                a.tables_out[(int64_t)j * a.width + len / P] = p;
+                a.copies[slot] = make_int4(s_last[j], p, len % P, 0);
+                atomicSub(&a.refs_out[s_last[j]], 1);
+            } else {
+                a.tables_out[(int64_t)j * a.width + pages_of(len, P) + t - (slot >= 0)] = p;
+            }
+        }
+    }
+    if (rank == 0) {
+        for (int j = tid; j < a.n_out; j += PG_THREADS) {
+            const int len = max(s_len[j], 0);
+            const bool grows = ok && s_len[j] >= 0 && !(a.frozen && a.frozen[j]);
+            a.lens_out[j] = len + (grows ? a.n_new : 0);
+        }
+        if (tid == 0) {
+            a.result[0] = ok ? base : 0;
+            a.result[1] = max(base - free_pages, 0);
+            a.result[2] = s_over;
+            a.result[3] = s_allbad;
+            *a.n_copies = ok ? cbase : 0;
+        }
+    }
+    cluster.sync();  // no CTA leaves while another reads its shared memory
+}
+
+// Compaction: used pages at or above the number of used pages go to the free pages below
+// it, the k-th to the k-th.
+__global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(const PagesArgs a)
+{
+    cg::cluster_group cluster = cg::this_cluster();
+    __shared__ int s_used[PG_WARPS], s_sh[PG_WARPS + 1], s_mv[PG_SLICES], s_ho[PG_SLICES], s_cut[2];
+    const int rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int gw = rank * PG_WARPS + warp, gt = rank * PG_THREADS + tid;
+    const int per = (a.n_pages + PG_SLICES - 1) / PG_SLICES;
+    const int64_t lo = (int64_t)gw * per;
+    const int n_slice = (int)max((int64_t)0, min((int64_t)per, a.n_pages - lo));
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    int n = 0;
+    for (int i = lane; i < n_slice; i += 32) n += a.refs_in[lo + i] > 0;
+    n = __reduce_add_sync(FULLMASK, n);
+    if (lane == 0) s_used[warp] = n;
+    if (tid < 2) s_cut[tid] = 0;
+    cluster.sync();
+    int used;
+    const int mine = tid < PG_SLICES ? *cluster.map_shared_rank(&s_used[tid % PG_WARPS], tid / PG_WARPS) : 0;
+    pg_scan(mine, &used, s_sh);
+    // pages to move and holes of every slice; the one that holds the border is counted again
+    const int cut = used / per;  // its slice (every page used: none)
+    for (int64_t p = (int64_t)cut * per + tid; p < min((int64_t)(cut + 1) * per, (int64_t)a.n_pages); p += PG_THREADS) {
+        const bool u = a.refs_in[p] > 0;
+        if (u && p >= used) atomicAdd(&s_cut[0], 1);
+        if (!u && p < used) atomicAdd(&s_cut[1], 1);
+    }
+    __syncthreads();
+    int moves = 0, holes = 0;
+    if (tid < PG_SLICES) {
+        if (tid == cut) {
+            moves = s_cut[0];
+            holes = s_cut[1];
+        } else if (tid > cut) {
+            moves = mine;
+        } else {
+            holes = (int)max((int64_t)0, min((int64_t)per, (int64_t)a.n_pages - (int64_t)tid * per)) - mine;
+        }
+    }
+    int total, htotal;
+    const int mo = pg_scan(moves, &total, s_sh), ho = pg_scan(holes, &htotal, s_sh);
+    if (tid < PG_SLICES) {
+        s_mv[tid] = mo;
+        s_ho[tid] = ho;
+    }
+    __syncthreads();
+    int m0 = s_mv[gw], h0 = s_ho[gw];
+    for (int i0 = 0; i0 < n_slice; i0 += 32) {
+        const int p = (int)lo + i0 + lane;
+        const bool in = i0 + lane < n_slice;
+        const int refs = in ? a.refs_in[p] : 0;
+        const bool mv = in && refs > 0 && p >= used, hole = in && refs <= 0 && p < used;
+        const unsigned mb = __ballot_sync(FULLMASK, mv), hb = __ballot_sync(FULLMASK, hole);
+        if (mv) a.moves[2 * (m0 + __popc(mb & ((1u << lane) - 1)))] = p;
+        if (hole) a.moves[2 * (h0 + __popc(hb & ((1u << lane) - 1))) + 1] = p;
+        m0 += __popc(mb);
+        h0 += __popc(hb);
+        if (in && !mv) a.page_map[p] = refs > 0 ? p : -1;
+        if (in && !mv && !hole) a.refs_out[p] = refs > 0 ? refs : 0;
+    }
+    cluster.sync();  // the moves are listed
+    for (int k = gt; k < total; k += PG_CLUSTER * PG_THREADS) {
+        const int from = __ldcg(a.moves + 2 * k), to = __ldcg(a.moves + 2 * k + 1);
+        const int refs = a.refs_in[from];
+        a.page_map[from] = to;
+        a.refs_out[to] = refs;
+        a.refs_out[from] = 0;
+    }
+    if (gt == 0) {
+        a.result[0] = used;
+        a.result[1] = total;
+        a.result[2] = 0;
+        a.result[3] = 0;
+    }
+}
+
+// One chunk of a page: the first `fill` positions of its segments.
+template <class V>
+__device__ __forceinline__ void copy_chunk(const PoolArg &q, int from, int to, int fill, int chunk)
+{
+    const uint32_t cols = (uint32_t)fill * q.token_vecs, all = cols * (uint32_t)q.segs;
+    const char *src = q.data + (int64_t)from * q.page_stride;
+    char *dst = q.data + (int64_t)to * q.page_stride;
+    const uint32_t c0 = (uint32_t)chunk * (PC_THREADS * PC_VECS) + threadIdx.x;
+    V v[PC_VECS];
+    int64_t off[PC_VECS];
+#pragma unroll
+    for (int i = 0; i < PC_VECS; i++) {
+        const uint32_t c = c0 + i * PC_THREADS;
+        if (c < all) {
+            const uint32_t seg = c / cols;
+            off[i] = (int64_t)seg * q.seg_stride + (int64_t)(c - seg * cols) * (int64_t)sizeof(V);
+            v[i] = *(const V *)(src + off[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PC_VECS; i++)
+        if (c0 + i * PC_THREADS < all) *(V *)(dst + off[i]) = v[i];
+}
+
+// The listed pages' contents, pool by pool: a fork copies the filled positions of its
+// copies, a compaction whole pages (and renames the tables' entries).
+template <bool FORK>
+__global__ void __launch_bounds__(PC_THREADS) pages_copy_kernel(const PagesArgs a, const PoolArgs pools)
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if constexpr (!FORK) {
+        for (int i = blockIdx.x; i < a.n_in; i += gridDim.x) {
+            const int64_t most = (int64_t)a.width * a.page_tokens;
+            const int raw = a.lens_in[i];
+            const int len = raw < 0 ? 0 : (int)min((int64_t)raw, most);
+            int bad = threadIdx.x == 0 && len != raw;
+            for (int c = threadIdx.x; c < pages_of(len, a.page_tokens); c += PC_THREADS) {
+                const int64_t o = (int64_t)i * a.width + c;
+                int p = a.tables_in[o];
+                if (p >= 0 && p < a.n_pages) {
+                    p = __ldcg(a.page_map + p);
+                    bad += p < 0;
+                } else {
+                    bad++;
+                }
+                a.tables_out[o] = p;
+            }
+            if (bad) atomicAdd(&a.result[3], bad);
+        }
+    }
+    const int n = FORK ? *a.n_copies : a.result[1];
+    const int64_t units = (int64_t)n * pools.n * pools.chunks;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int chunk = (int)(u % pools.chunks);
+        const int64_t rest = u / pools.chunks;
+        const PoolArg &q = pools.p[rest % pools.n];
+        const int64_t k = rest / pools.n;
+        int from, to, fill;
+        if constexpr (FORK) {
+            const int4 c = __ldcg(a.copies + k);
+            from = c.x, to = c.y, fill = c.z;
+        } else {
+            from = __ldcg(a.moves + 2 * k), to = __ldcg(a.moves + 2 * k + 1), fill = a.page_tokens;
+        }
+        if (q.width == 16) copy_chunk<uint4>(q, from, to, fill, chunk);
+        else if (q.width == 4) copy_chunk<uint32_t>(q, from, to, fill, chunk);
+        else copy_chunk<uint8_t>(q, from, to, fill, chunk);
+    }
+}
+
+int pages_chunk_vecs() { return PC_THREADS * PC_VECS; }
+
+int pages_fork_smem(int n_in, int n_out) { return (n_in + 4 * (n_in > n_out ? n_in : n_out)) * (int)sizeof(int); }
+
+template <bool FORK>
+static cudaError_t launch_copy(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s)
+{
+    int64_t work = (int64_t)a.max_copies * pools.n * pools.chunks;
+    if (!FORK && work < a.n_in) work = a.n_in;
+    if (work == 0) return cudaSuccess;
+    const int64_t most = (int64_t)sms * 8;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(work < most ? work : most));
+    cfg.blockDim = dim3(PC_THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, pages_copy_kernel<FORK>, a, pools);
+}
+
+cudaError_t launch_pages_fork(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s)
+{
+    const int smem = pages_fork_smem(a.n_in, a.n_out);
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(pages_fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+    }
+    pages_fork_kernel<<<PG_CLUSTER, PG_THREADS, smem, s>>>(a);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || a.n_new == 0) return e;
+    return launch_copy<true>(a, pools, sms, s);
+}
+
+cudaError_t launch_pages_compact(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s)
+{
+    pages_compact_kernel<<<PG_CLUSTER, PG_THREADS, 0, s>>>(a);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    return launch_copy<false>(a, pools, sms, s);
+}
+
+}  // namespace g4s

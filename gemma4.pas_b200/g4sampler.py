@@ -55,6 +55,56 @@ class Outputs(ctypes.Structure):
                 ("full_probs", c_void_p)]
 
 
+class BeamParams(ctypes.Structure):
+    """g4s_beam_params, 64 bytes."""
+
+    _fields_ = [("beams", c_int32), ("n_out", c_int32), ("temperature", c_double), ("length_alpha", c_double),
+                ("pad_token", c_int32), ("n_eos", c_int32), ("eos", c_int32 * 8)]
+
+
+class BeamState(ctypes.Structure):
+    """g4s_beam_state: device pointers of scores (fp32), lens (int32 or 0) and done (uint8 or 0)."""
+
+    _fields_ = [("scores", c_void_p), ("lens", c_void_p), ("done", c_void_p)]
+
+
+class BeamTensor(ctypes.Structure):
+    """g4s_beam_tensor: row r's state is segs0 x segs1 segments of seg_bytes (all strides in bytes)."""
+
+    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("row_stride", c_int64), ("segs0", c_int32),
+                ("stride0", c_int64), ("segs1", c_int32), ("stride1", c_int64), ("seg_bytes", c_int64)]
+
+
+class PagePool(ctypes.Structure):
+    """g4s_page_pool: page p's segments at data + p * page_stride + s * seg_stride (bytes)."""
+
+    _fields_ = [("data", c_void_p), ("page_stride", c_int64), ("segs", c_int32), ("seg_stride", c_int64),
+                ("token_bytes", c_int64)]
+
+
+class PageCache(ctypes.Structure):
+    """g4s_page_cache; build it with page_cache(), which keeps the pool list alive."""
+
+    _fields_ = [("page_tokens", c_int32), ("n_pages", c_int32), ("max_seq_pages", c_int32), ("n_pools", c_int32),
+                ("pools", POINTER(PagePool))]
+
+
+class PageTables(ctypes.Structure):
+    """g4s_page_tables: device pointers of the tables, lengths and page counts (int32)."""
+
+    _fields_ = [("tables", c_void_p), ("lens", c_void_p), ("refs", c_void_p)]
+
+
+class BeamPages(ctypes.Structure):
+    """g4s_beam_pages: the paged cache of a beam_step."""
+
+    _fields_ = [("cache", POINTER(PageCache)), ("in_", PageTables), ("out", PageTables), ("n_new", c_int32),
+                ("result", c_void_p)]
+
+
+BEAM_MAX, BEAM_MAX_OUT, BEAM_MAX_EOS, BEAM_MAX_TENSORS = 32, 64, 8, 32
+PAGES_MAX_POOLS, PAGES_MAX_SEQS = 96, 8192
+
 # every entry point include/g4sampler.h declares, with (restype, argtypes)
 SIGNATURES = {
     "g4s_version": (c_int32, []),
@@ -93,6 +143,18 @@ SIGNATURES = {
     "g4s_shard_init": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_void_p]),
     "g4s_shard_sample": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int64, POINTER(Params), c_int32,
                                    c_float, c_void_p, c_void_p, POINTER(Outputs), c_void_p]),
+    "g4s_beam_params_defaults": (None, [POINTER(BeamParams)]),
+    "g4s_beam_select": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int64, c_float,
+                                  POINTER(BeamParams), POINTER(BeamState), POINTER(BeamState), c_void_p, c_void_p,
+                                  c_void_p]),
+    "g4s_beam_reorder": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, POINTER(BeamTensor), c_int32, c_void_p]),
+    "g4s_pages_fork": (c_int32, [c_void_p, POINTER(PageCache), c_int32, POINTER(PageTables), c_int32, c_void_p,
+                                 c_int32, c_void_p, POINTER(PageTables), c_void_p, c_void_p]),
+    "g4s_pages_compact": (c_int32, [c_void_p, POINTER(PageCache), c_int32, POINTER(PageTables), POINTER(PageTables),
+                                    c_void_p, c_void_p, c_void_p, c_void_p]),
+    "g4s_beam_step": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int64, c_float,
+                                POINTER(BeamParams), POINTER(BeamState), POINTER(BeamState), c_void_p, c_void_p,
+                                POINTER(BeamTensor), c_int32, POINTER(BeamPages), c_void_p]),
     "g4s_vpk_open": (c_int32, [c_char_p, c_char_p, c_char_p, POINTER(c_void_p)]),
     "g4s_vpk_close": (c_int32, [c_void_p]),
     "g4s_vpk_tensor_count": (c_int32, [c_void_p]),
@@ -158,6 +220,39 @@ class G4SError(RuntimeError):
 
 def make_params(temperature=1.0, top_k=64, top_p=0.95, repetition_penalty=1.0) -> Params:
     return Params(float(temperature), int(top_k), float(top_p), float(repetition_penalty))
+
+
+def make_beam_params(beams=4, n_out=None, temperature=1.0, length_alpha=0.0, pad_token=0, eos=(1, 106, 50)) -> BeamParams:
+    """g4s_beam_params; n_out None: as many continuations as beams."""
+    if len(eos) > BEAM_MAX_EOS:
+        raise ValueError(f"{len(eos)} end tokens: at most {BEAM_MAX_EOS}")
+    p = BeamParams(int(beams), int(beams if n_out is None else n_out), float(temperature), float(length_alpha),
+                   int(pad_token), len(eos))
+    for i, t in enumerate(eos):
+        p.eos[i] = int(t)
+    return p
+
+
+def beam_tensors(tensors):
+    """ctypes array of BeamTensor from a sequence; an array this function made is passed through."""
+    if tensors is None or (isinstance(tensors, ctypes.Array) and tensors._type_ is BeamTensor):
+        return tensors
+    return (BeamTensor * len(tensors))(*tensors)
+
+
+def page_cache(pools, page_tokens: int, n_pages: int, max_seq_pages: int) -> PageCache:
+    """g4s_page_cache over a sequence of PagePool."""
+    arr = (PagePool * max(1, len(pools)))(*pools)
+    c = PageCache(page_tokens, n_pages, max_seq_pages, len(pools), ctypes.cast(arr, POINTER(PagePool)))
+    c.pool_array = arr  # the struct holds an address only
+    return c
+
+
+def beam_pages(cache: PageCache, in_: PageTables, out: PageTables, n_new: int, result_ptr: int) -> BeamPages:
+    """g4s_beam_pages of a beam_step."""
+    p = BeamPages(ctypes.pointer(cache), in_, out, n_new, result_ptr)
+    p.cache_kept = cache
+    return p
 
 
 def params_array(rows):
@@ -316,6 +411,59 @@ class Sampler:
                                         c_void_p(logits_ptr) if logits_ptr else None,
                                         c_void_p(stream) if stream else None)
         if check:
+            self._check(rc)
+        return rc
+
+    def beam_select(self, logits_ptr: int, dtype: int, groups: int, vocab: int, row_stride: int, softcap: float,
+                    params: BeamParams, before: BeamState, after: BeamState, parents_ptr: int, tokens_ptr: int,
+                    stream: int | None = None, check: bool = True) -> int:
+        """g4s_beam_select: each group's best continuations over beams x vocabulary."""
+        rc = self.lib.g4s_beam_select(self.h, logits_ptr, dtype, groups, vocab, row_stride, softcap, params, before,
+                                      after, parents_ptr, tokens_ptr, stream or None)
+        if check and rc != OK:
+            self._check(rc)
+        return rc
+
+    def beam_reorder(self, parents_ptr: int, groups: int, beams: int, tensors, stream: int | None = None,
+                     check: bool = True) -> int:
+        """g4s_beam_reorder: dense states by their parents (tensors: beam_tensors([...]))."""
+        arr = beam_tensors(tensors)
+        rc = self.lib.g4s_beam_reorder(self.h, parents_ptr, groups, beams, arr, len(arr), stream or None)
+        if check and rc != OK:
+            self._check(rc)
+        return rc
+
+    def pages_fork(self, cache: PageCache, n_in: int, tables_ptr: int, lens_ptr: int, refs_ptr: int, n_out: int,
+                   src_ptr: int, n_new: int, out_tables_ptr: int, out_lens_ptr: int, out_refs_ptr: int,
+                   result_ptr: int, frozen_ptr: int = 0, stream: int | None = None, check: bool = True) -> int:
+        """g4s_pages_fork: sequences continued, shared, freed and grown by src."""
+        rc = self.lib.g4s_pages_fork(self.h, cache, n_in, PageTables(tables_ptr, lens_ptr, refs_ptr), n_out, src_ptr,
+                                     n_new, frozen_ptr or None, PageTables(out_tables_ptr, out_lens_ptr, out_refs_ptr),
+                                     result_ptr, stream or None)
+        if check and rc != OK:
+            self._check(rc)
+        return rc
+
+    def pages_compact(self, cache: PageCache, n_seqs: int, tables_ptr: int, lens_ptr: int, refs_ptr: int,
+                      out_tables_ptr: int, out_refs_ptr: int, map_ptr: int, moves_ptr: int, result_ptr: int,
+                      stream: int | None = None, check: bool = True) -> int:
+        """g4s_pages_compact: used pages to the lowest ids."""
+        rc = self.lib.g4s_pages_compact(self.h, cache, n_seqs, PageTables(tables_ptr, lens_ptr, refs_ptr),
+                                        PageTables(out_tables_ptr, None, out_refs_ptr), map_ptr, moves_ptr, result_ptr,
+                                        stream or None)
+        if check and rc != OK:
+            self._check(rc)
+        return rc
+
+    def beam_step(self, logits_ptr: int, dtype: int, groups: int, vocab: int, row_stride: int, softcap: float,
+                  params: BeamParams, before: BeamState, after: BeamState, parents_ptr: int, tokens_ptr: int,
+                  tensors=None, pages: BeamPages | None = None, stream: int | None = None, check: bool = True) -> int:
+        """g4s_beam_step: the selection, then the dense states and the paged cache by its parents."""
+        arr = beam_tensors(tensors)
+        rc = self.lib.g4s_beam_step(self.h, logits_ptr, dtype, groups, vocab, row_stride, softcap, params, before,
+                                    after, parents_ptr, tokens_ptr, arr, len(arr) if arr is not None else 0, pages,
+                                    stream or None)
+        if check and rc != OK:
             self._check(rc)
         return rc
 

@@ -50,6 +50,13 @@ const
   G4S_SHARD_LIST      = 256;   { composites per row per shard list }
   G4S_SHARD_UID_BYTES = 128;
 
+  G4S_BEAM_MAX         = 32;
+  G4S_BEAM_MAX_OUT     = 64;
+  G4S_BEAM_MAX_EOS     = 8;
+  G4S_BEAM_MAX_TENSORS = 32;
+  G4S_PAGES_MAX_POOLS  = 96;
+  G4S_PAGES_MAX_SEQS   = 8192;
+
 type
   { Same layout as TSamplingParams (src/Gemma4.Model.pas:70-76): four 4-byte
     fields at offsets 0/4/8/12, so a TSamplingParams can be passed by address. }
@@ -86,6 +93,71 @@ type
   end;
   PG4STensorInfo = ^TG4STensorInfo;
   PG4SVpk = Pointer;
+
+  { Beam search (g4s_beam_params, 64 bytes; the state records hold device pointers). }
+  TG4SBeamParams = record
+    Beams: Int32;
+    NOut: Int32;
+    Temperature: Double;
+    LengthAlpha: Double;
+    PadToken: Int32;
+    NEos: Int32;
+    Eos: array[0..G4S_BEAM_MAX_EOS - 1] of Int32;
+  end;
+  PG4SBeamParams = ^TG4SBeamParams;
+
+  TG4SBeamState = record
+    Scores: PSingle;
+    Lens: PInt32;
+    Done: PByte;
+  end;
+  PG4SBeamState = ^TG4SBeamState;
+
+  TG4SBeamTensor = record
+    Src: Pointer;
+    Dst: Pointer;
+    RowStride: Int64;
+    Segs0: Int32;
+    Stride0: Int64;
+    Segs1: Int32;
+    Stride1: Int64;
+    SegBytes: Int64;
+  end;
+  PG4SBeamTensor = ^TG4SBeamTensor;
+
+  TG4SPagePool = record
+    Data: Pointer;
+    PageStride: Int64;
+    Segs: Int32;
+    SegStride: Int64;
+    TokenBytes: Int64;
+  end;
+  PG4SPagePool = ^TG4SPagePool;
+
+  TG4SPageCache = record
+    PageTokens: Int32;
+    NPages: Int32;
+    MaxSeqPages: Int32;
+    NPools: Int32;
+    Pools: PG4SPagePool;
+  end;
+  PG4SPageCache = ^TG4SPageCache;
+
+  TG4SPageTables = record
+    Tables: PInt32;
+    Lens: PInt32;
+    Refs: PInt32;
+  end;
+  PG4SPageTables = ^TG4SPageTables;
+
+  TG4SBeamPages = record
+    Cache: PG4SPageCache;
+    InTables: TG4SPageTables;
+    OutTables: TG4SPageTables;
+    NNew: Int32;
+    Result_: PInt32;
+  end;
+  PG4SBeamPages = ^TG4SBeamPages;
 
 function g4s_version(): Int32; cdecl; external G4SLib;
 procedure g4s_params_defaults(P: PG4SParams); cdecl; external G4SLib;
@@ -158,6 +230,29 @@ function g4s_shard_init(Ctx: PG4SCtx; World, Rank, VocabTotal: Int32;
 function g4s_shard_sample(Ctx: PG4SCtx; LogitsSlice: Pointer; DType, Rows: Int32;
   RowStride: Int64; Params: PG4SParams; ParamsStride: Int32; Softcap: Single;
   U: PDouble; OutTokens: PInt32; Extra: PG4SOutputs;
+  Stream: Pointer): Int32; cdecl; external G4SLib;
+
+{ Beam search: selection over beams x vocabulary, the states and the paged cache
+  by its parents, and the three in one call. }
+procedure g4s_beam_params_defaults(P: PG4SBeamParams); cdecl; external G4SLib;
+function g4s_beam_select(Ctx: PG4SCtx; Logits: Pointer; DType, Groups, Vocab: Int32;
+  RowStride: Int64; Softcap: Single; Params: PG4SBeamParams;
+  InState, OutState: PG4SBeamState; OutParents, OutTokens: PInt32;
+  Stream: Pointer): Int32; cdecl; external G4SLib;
+function g4s_beam_reorder(Ctx: PG4SCtx; Parents: PInt32; Groups, Beams: Int32;
+  Tensors: PG4SBeamTensor; NTensors: Int32; Stream: Pointer): Int32; cdecl;
+  external G4SLib;
+function g4s_pages_fork(Ctx: PG4SCtx; Cache: PG4SPageCache; NIn: Int32;
+  InTables: PG4SPageTables; NOut: Int32; Src: PInt32; NNew: Int32; Frozen: PByte;
+  OutTables: PG4SPageTables; Res: PInt32; Stream: Pointer): Int32; cdecl;
+  external G4SLib;
+function g4s_pages_compact(Ctx: PG4SCtx; Cache: PG4SPageCache; NSeqs: Int32;
+  InTables, OutTables: PG4SPageTables; PageMap, Moves, Res: PInt32;
+  Stream: Pointer): Int32; cdecl; external G4SLib;
+function g4s_beam_step(Ctx: PG4SCtx; Logits: Pointer; DType, Groups, Vocab: Int32;
+  RowStride: Int64; Softcap: Single; Params: PG4SBeamParams;
+  InState, OutState: PG4SBeamState; OutParents, OutTokens: PInt32;
+  Tensors: PG4SBeamTensor; NTensors: Int32; Pages: PG4SBeamPages;
   Stream: Pointer): Int32; cdecl; external G4SLib;
 
 { The VPK weight archive (TWeightStore): open, look up, read, load the LM head. }

@@ -393,6 +393,174 @@ int32_t g4s_vpk_verify(const g4s_vpk *vpk, const char *entry_path);
 int32_t g4s_vpk_load_lmhead(const g4s_vpk *vpk, int32_t device, uint8_t *nibbles, uint16_t *scales, int32_t max_vocab,
                             int32_t *out_vocab, int32_t *out_hidden, void *stream);
 
+/*
+ * Beam search (no counterpart in the reference: TModel.Generate,
+ * src/Gemma4.Model.pas:2829-2938, keeps one sequence).  A prompt is a group of
+ * `beams` adjacent rows.  One decode step: the model's logits of every row,
+ * g4s_beam_select, then the selected parents move the rows' states
+ * (g4s_beam_reorder for dense ones, g4s_pages_fork for a paged cache);
+ * g4s_beam_step is these in one call.  All pointers are device memory except
+ * the structs and the pool list; calls are asynchronous on `stream` (NULL: the
+ * context stream) and may be captured.  They share the context's workspace:
+ * calls of one context that may overlap on the GPU (two streams, two captured
+ * graphs) need a context each.
+ */
+#define G4S_BEAM_MAX         32  /* beams a group                      */
+#define G4S_BEAM_MAX_OUT     64  /* continuations kept a group         */
+#define G4S_BEAM_MAX_EOS      8
+#define G4S_BEAM_MAX_TENSORS 32  /* tensors of one g4s_beam_reorder    */
+#define G4S_PAGES_MAX_POOLS  96
+#define G4S_PAGES_MAX_SEQS 8192
+
+typedef struct g4s_beam_params {
+    int32_t beams;          /* rows a group, 1..G4S_BEAM_MAX                          */
+    int32_t n_out;          /* continuations kept a group, 1..G4S_BEAM_MAX_OUT        */
+    double  temperature;    /* 1e-6..1e6                                              */
+    double  length_alpha;   /* 0..8: ranked by score / max(length, 1)^length_alpha    */
+    int32_t pad_token;      /* the token an ended beam continues with                 */
+    int32_t n_eos;          /* end tokens in eos[], 0..G4S_BEAM_MAX_EOS               */
+    int32_t eos[G4S_BEAM_MAX_EOS];
+} g4s_beam_params;
+
+/* beams / n_out = 4, temperature 1, length_alpha 0, pad_token 0 and the
+   reference's end tokens 1, 106, 50 (src/Gemma4.Types.pas:65-67). */
+void g4s_beam_params_defaults(g4s_beam_params *p);
+
+/* State of the beams, one element a row (in: groups * beams, out: groups * n_out). */
+typedef struct g4s_beam_state {
+    float   *scores;   /* sum of log-probabilities; -inf (or NaN): no beam          */
+    int32_t *lens;     /* tokens generated; may be NULL where length_alpha is 0      */
+    uint8_t *done;     /* != 0: the beam has ended; NULL: none has / not wanted      */
+} g4s_beam_state;
+
+/*
+ * Per group, the n_out best continuations of its beams.  A beam's token i has
+ *   x_i = s(l_i) / T,  s(l) = softcap * tanh(l / softcap), or l for softcap <= 0,
+ *   score = scores[beam] + x_i - log sum_j exp(x_j),
+ * where a logit that is NaN or at or below -1e30 is masked (no candidate, no
+ * mass; a row without any other has no candidate) and +inf counts as the
+ * largest finite number.  An ended beam has one continuation: pad_token at its
+ * own score and length.  Order: score / max(length after the token,
+ * 1)^length_alpha, descending, computed in 64 bits; then the lower beam; within
+ * a beam the larger logit, then the lower id.  Places that no continuation
+ * fills get score -inf, parent and token -1, length 0, done 0.
+ *   logits        rows x row_stride elements, rows = groups * params->beams
+ *   out_parents   [groups * n_out] the row continued (0..rows-1)
+ *   out_tokens    [groups * n_out]
+ *   in, out       out may be in (the same pointers) when n_out == beams; other
+ *                 overlaps are refused.  out->lens needs in->lens.
+ * softcap: 0 or below (none), or 1e-6..1e6.
+ */
+int32_t g4s_beam_select(g4s_ctx *ctx, const void *logits, int32_t dtype, int32_t groups, int32_t vocab,
+                        int64_t row_stride, float softcap, const g4s_beam_params *params, const g4s_beam_state *in,
+                        const g4s_beam_state *out, int32_t *out_parents, int32_t *out_tokens, void *stream);
+
+/* A dense state of the rows: row r's bytes are segs0 x segs1 segments of
+   seg_bytes at data + r * row_stride + i * stride0 + j * stride1 (bytes, >= 0).
+   For caches [layers][rows][heads][max_len][dim]: row_stride of one row's block,
+   segs0 the layers, segs1 the heads, seg_bytes the positions in use. */
+typedef struct g4s_beam_tensor {
+    const void *src;
+    void       *dst;        /* src itself (in place), or memory that shares no byte with it */
+    int64_t     row_stride;
+    int32_t     segs0;
+    int64_t     stride0;
+    int32_t     segs1;
+    int64_t     stride1;
+    int64_t     seg_bytes;
+} g4s_beam_tensor;
+
+/* dst row j <- src row parents[j], for every tensor, in one launch.  A parent
+   outside the row's own group (-1 among them) leaves the row as it was.
+   Segments must not overlap one another.  Fastest where all addresses, strides
+   and seg_bytes are multiples of 16, then of 4. */
+int32_t g4s_beam_reorder(g4s_ctx *ctx, const int32_t *parents, int32_t groups, int32_t beams,
+                         const g4s_beam_tensor *tensors, int32_t n_tensors, void *stream);
+
+/* One pool of pages (a layer's K or V): page p holds `segs` segments at data +
+   p * page_stride + s * seg_stride, each page_tokens positions of token_bytes. */
+typedef struct g4s_page_pool {
+    void   *data;
+    int64_t page_stride;
+    int32_t segs;
+    int64_t seg_stride;
+    int64_t token_bytes;
+} g4s_page_pool;
+
+typedef struct g4s_page_cache {
+    int32_t page_tokens;        /* positions a page                                   */
+    int32_t n_pages;            /* pages a pool; page ids are the same in every pool  */
+    int32_t max_seq_pages;      /* entries of a table's row                           */
+    int32_t n_pools;            /* 0: only tables and counts                          */
+    const g4s_page_pool *pools; /* host array                                         */
+} g4s_page_cache;
+
+/* Tables of a paged cache: sequence i's positions 0..lens[i]-1 lie in the pages
+   tables[i * max_seq_pages + 0 ..]; refs[p] counts the sequences (and other
+   holders) of page p, 0 or below: free. */
+typedef struct g4s_page_tables {
+    int32_t *tables;
+    int32_t *lens;
+    int32_t *refs;
+} g4s_page_tables;
+
+/*
+ * Replaces the n_in sequences of `in` by n_out sequences of `out`: sequence j
+ * continues src[j] (its pages shared, not copied), or is empty for src[j] < 0.
+ * Pages that no sequence holds any more become free: forking, freeing
+ * (src -1) and growing (src[j] = j) are this one call.  With n_new > 0 each
+ * sequence that is not empty (nor frozen[j] != 0; frozen may be NULL) gets
+ * room for n_new more positions, counted in its length: a partly filled last
+ * page that others hold too is copied (of w such sequences and r holders, the
+ * first min(w, r - 1) get a copy; only filled positions are copied), whole new
+ * pages are added.  Pages are taken in ascending id, sequences in order, a
+ * copy before the sequence's new pages.  Only the table entries in use and the
+ * positions copied are written.
+ *   result  int32 [4]: pages taken; pages missing; sequences whose table is
+ *           too short for n_new; bad inputs (src >= n_in, a length outside
+ *           0..max_seq_pages * page_tokens -- its sequence becomes empty --, a
+ *           page id outside the pool -- kept, not counted).  Unless the last
+ *           three are 0 no page is taken and no length grows: `out` is the fork
+ *           alone.
+ * out->tables is other memory than in->tables; lens and refs may be the same.
+ * At most min(max_rows, G4S_PAGES_MAX_SEQS) sequences; tables and lens may be
+ * NULL for none.
+ */
+int32_t g4s_pages_fork(g4s_ctx *ctx, const g4s_page_cache *cache, int32_t n_in, const g4s_page_tables *in,
+                       int32_t n_out, const int32_t *src, int32_t n_new, const uint8_t *frozen,
+                       const g4s_page_tables *out, int32_t *result, void *stream);
+
+/*
+ * Moves the used pages (refs > 0) to the ids 0..used-1: those at or above
+ * `used` go, in ascending order, to the free ids below it.  `out` may be `in`;
+ * lens is only read (in->lens).
+ *   page_map  [n_pages] the new id of each page, -1 for a free one (for holders
+ *             besides the tables)
+ *   moves     [n_pages] (from, to) pairs; only the moved ones are written
+ *   result    int32 [4]: pages used; pages moved; 0; bad inputs (lengths out
+ *             of range, taken as the nearest in range; table entries outside the
+ *             pool, kept; entries of a free page, set to -1)
+ */
+int32_t g4s_pages_compact(g4s_ctx *ctx, const g4s_page_cache *cache, int32_t n_seqs, const g4s_page_tables *in,
+                          const g4s_page_tables *out, int32_t *page_map, int32_t *moves, int32_t *result,
+                          void *stream);
+
+/* The paged cache of a g4s_beam_step. */
+typedef struct g4s_beam_pages {
+    const g4s_page_cache *cache;
+    g4s_page_tables in, out;    /* groups * beams sequences, out as in g4s_pages_fork */
+    int32_t  n_new;             /* positions to make room for (ended beams get none where out->done is set) */
+    int32_t *result;
+} g4s_beam_pages;
+
+/* One step of beam search: g4s_beam_select (n_out == beams), then by its
+   parents g4s_beam_reorder of `tensors` (NULL: none) and g4s_pages_fork of
+   `pages` (NULL: none).  Arguments are checked before anything is launched. */
+int32_t g4s_beam_step(g4s_ctx *ctx, const void *logits, int32_t dtype, int32_t groups, int32_t vocab,
+                      int64_t row_stride, float softcap, const g4s_beam_params *params, const g4s_beam_state *in,
+                      const g4s_beam_state *out, int32_t *out_parents, int32_t *out_tokens,
+                      const g4s_beam_tensor *tensors, int32_t n_tensors, const g4s_beam_pages *pages, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
