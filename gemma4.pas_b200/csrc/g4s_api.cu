@@ -1387,7 +1387,7 @@ static bool aliasing_ok(const void *in, const void *out, size_t in_bytes, size_t
 
 static int pow2_at_least(int n)
 {
-    int p = 2;
+    int p = 4;
     while (p < n) p <<= 1;
     return p;
 }
@@ -1436,16 +1436,10 @@ static int32_t beam_select_args(g4s_ctx *ctx, const char *who, const void *logit
     a.beams = p->beams;
     a.vocab = vocab;
     a.n_out = p->n_out;
-    const int unit = beam_unit_logits(dtype), units = (int)ceil_div(vocab, unit);
-    a.upi = (int)ceil_div(units, BEAM_MAX_ITEMS);
-    a.ipr = (int)ceil_div(units, a.upi);
     a.pe = pow2_at_least(p->beams * p->n_out);
-    a.pc = pow2_at_least(p->n_out * (p->n_out + 1) / 2);
+    a.pc = std::max(512, pow2_at_least(p->n_out * (p->n_out + 1) / 2));
     a.softcap = softcap > 0.0f ? softcap : 0.0f;
-    a.invcap = softcap > 0.0f ? 1.0f / softcap : 0.0f;
     a.k64 = 1.4426950408889634074 / p->temperature;
-    a.k = (float)a.k64;
-    a.temperature = p->temperature;
     a.alpha = p->length_alpha;
     a.pad_token = p->pad_token;
     a.n_eos = p->n_eos;

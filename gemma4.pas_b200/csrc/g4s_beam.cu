@@ -9,17 +9,16 @@
 //   scores[w] + x_i - lse,   ranked by  score / max(len, 1)^alpha,
 // and a prompt's n_out best continuations over its beams are wanted.  Within a
 // beam the rank is increasing in the raw logit, so only raw comparisons order
-// a beam's tokens; the beams' own scores meet in 64 bits, for the few tokens
-// that can be among the best.
+// a beam's tokens; the beams' scores meet in pairs of fp32 numbers, for the
+// few tokens that can be among the best.
 //
-// beam_stream_kernel: one pass over the logits.  An item is a whole number of
-//   2 KiB units of one row (one unit up to 512 units a row); a warp reduces it
-//   to (largest raw logit m, its softcapped value c, S = sum 2^((s_i - c) k)),
-//   k = log2(e) / T.  The difference s_i - c is taken before the product with
-//   k, so that k's rounding acts on the distance from the maximum only.
+// beam_stream_kernel: one pass over the logits.  An item is `upi` 2 KiB units of one
+//   row; a warp reduces it to (m, ref, S): the largest raw logit, a reference in
+//   units of 2 (ref = s(m) k with the softcap, else m), and
+//   S = sum 2^(s_i k - ref) (2^((l_i - ref) k)), k = log2(e) / T.
 // beam_combine_kernel: one CTA a prompt.
-//   1. a warp a beam: lse from the items in 64 bits, and the beam's n_out
-//      items with the largest (m, then lowest item);
+//   1. a warp a beam: the row's sum from its items (as pairs), and its n_out items with the
+//      largest (m, then lowest item);
 //   2. those items' best tokens ranked over the beams: the n_out best tokens
 //      lie in the n_out items that rank first (each item that ranks before
 //      another holds a token that beats all of the other's);
@@ -30,11 +29,14 @@
 
 namespace g4s {
 
-constexpr int BS_THREADS = 256;  // CTA of the streaming pass
-constexpr int BC_THREADS = 512;  // CTA of the combine
+constexpr int BS_THREADS = 128;  // CTA of the streaming pass
+constexpr int BS_CTAS = 6;       // of them on an SM: 80 registers a thread, 32 KiB a CTA
+constexpr int BS_STAGES = 2;     // loads a warp's ring in shared memory holds
+constexpr int BS_NV = 8;         // 16-byte vectors a lane and load (4 KiB, two units)
+constexpr int BC_THREADS = 1024; // CTA of the combine
 constexpr int BC_WARPS = BC_THREADS / 32;
-constexpr int BNV = 4;           // 16-byte vectors a lane and unit (2 KiB a unit)
 constexpr int BIPL = BEAM_MAX_ITEMS / 32;  // a row's items a lane of its warp
+constexpr int BNV = 4;           // 16-byte vectors a lane and unit (2 KiB a unit)
 
 template <int DT>
 struct BeamGeo {
@@ -43,15 +45,23 @@ struct BeamGeo {
     static constexpr int UNIT = 32 * EPL;   // 512 fp32 or 1024 bf16 logits
 };
 
-int beam_unit_logits(int dtype) { return dtype == G4S_F32 ? BeamGeo<G4S_F32>::UNIT : BeamGeo<G4S_BF16>::UNIT; }
-
 // A masked logit (NaN, or at or below -1e30 as on the top-K path) is -inf; +inf counts
-// as the largest finite number, so that differences stay defined; -0 is +0.
+// as the type's largest finite number, so that differences stay defined; -0 is +0.
+template <int DT>
+__device__ __forceinline__ float beam_max()
+{
+    return __uint_as_float(DT == G4S_BF16 ? 0x7f7f0000u : 0x7f7fffffu);
+}
+template <int DT>
 __device__ __forceinline__ float beam_raw(float v)
 {
-    return v > -1e30f ? fminf(v, 3.402823466e38f) + 0.0f : -__uint_as_float(0x7f800000u);
+    return v > -1e30f ? fminf(v, beam_max<DT>()) + 0.0f : -__uint_as_float(0x7f800000u);
 }
-__device__ __forceinline__ uint32_t beam_key(float v) { return cand_key(beam_raw(v)); }
+template <int DT>
+__device__ __forceinline__ uint32_t beam_key(float v)
+{
+    return cand_key(beam_raw<DT>(v));
+}
 
 // cap * tanh(v / cap) in fp32: the polynomial up to |q| = 1, 1 - 2 / (e^2q + 1) beyond
 // (2 / (e^2q + 1) < 0.24 there, so the approximate exponential and quotient cost less
@@ -69,11 +79,11 @@ __device__ __forceinline__ float beam_soft(float v, const BeamArgs &a)
 // Rows that are not 16-byte aligned are gathered element by element into the same places,
 // so that a row's sums do not depend on its alignment.
 template <int DT, bool VEC>
-__device__ __forceinline__ void load_unit(const char *p, int lane, uint4 (&r)[BNV])
+__device__ __forceinline__ void load_unit(const char *p, int lane, uint4 (&r)[BS_NV])
 {
     using T = DtypeTraits<DT>;
 #pragma unroll
-    for (int j = 0; j < BNV; j++) {
+    for (int j = 0; j < BS_NV; j++) {
         const int e0 = (j * 32 + lane) * T::VW;
         if constexpr (VEC) {
             r[j] = ld_stream_v4(p + (int64_t)e0 * T::ESIZE);
@@ -91,192 +101,409 @@ __device__ __forceinline__ void load_unit(const char *p, int lane, uint4 (&r)[BN
     }
 }
 
-struct UnitStat {
-    float m, c, S;
-};
-
-// Any unit, element by element: masked logits, |q| > 1, a row's ragged end.
-template <int DT, bool CAP>
-__device__ __forceinline__ UnitStat unit_general(const char *p, int n, int lane, const BeamArgs &a)
+// Two fp32 numbers in a 64-bit register: the packed operations' operands.  two() is volatile
+// so that a constant stays in its register instead of being rebuilt at every use.
+__device__ __forceinline__ uint64_t two(float x)
 {
-    const float NEG_INF = -__uint_as_float(0x7f800000u);
-    float mx = NEG_INF;
-#pragma unroll 4
-    for (int i = lane; i < n; i += 32) mx = fmaxf(mx, beam_raw(DtypeTraits<DT>::load1(p, i)));
-    UnitStat u{warp_max_redux(mx), 0.0f, 0.0f};
-    if (u.m == NEG_INF) return u;
-    u.c = beam_soft<CAP>(u.m, a);
-    float s = 0.0f;
-#pragma unroll 4
-    for (int i = lane; i < n; i += 32) {
-        const float v = beam_raw(DtypeTraits<DT>::load1(p, i));
-        const float e = ex2_approx((beam_soft<CAP>(v, a) - u.c) * a.k);
-        s += v == NEG_INF ? 0.0f : e;
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(FULLMASK, s, d);
-    u.S = s;
-    return u;
+    uint64_t r;
+    asm volatile("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t two(float x, float y)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
 }
 
-// A whole unit from registers; false when an element needs unit_general.
-template <int DT, bool CAP>
-__device__ __forceinline__ bool unit_fast(const uint4 (&r)[BNV], const BeamArgs &a, UnitStat &u)
+// This lane's largest and smallest logit of a load; a NaN comes through.
+template <int DT>
+__device__ __forceinline__ float lane_max(const uint4 (&r)[BS_NV])
+{
+    if constexpr (DT == G4S_BF16) {
+        uint32_t x = bmax2_nan(bmax2_nan(r[0].x, r[0].y), bmax2_nan(r[0].z, r[0].w));
+#pragma unroll
+        for (int j = 1; j < BS_NV; j++) x = bmax2_nan(x, bmax2_nan(bmax2_nan(r[j].x, r[j].y), bmax2_nan(r[j].z, r[j].w)));
+        return fmax_nan(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    } else {
+        float m = __uint_as_float(r[0].x);
+#pragma unroll
+        for (int j = 0; j < BS_NV; j++)
+            m = fmax3_nan(fmax3_nan(m, __uint_as_float(r[j].x), __uint_as_float(r[j].y)), __uint_as_float(r[j].z),
+                          __uint_as_float(r[j].w));
+        return m;
+    }
+}
+template <int DT>
+__device__ __forceinline__ float lane_min(const uint4 (&r)[BS_NV])
+{
+    if constexpr (DT == G4S_BF16) {
+        uint32_t x = bmin2_nan(bmin2_nan(r[0].x, r[0].y), bmin2_nan(r[0].z, r[0].w));
+#pragma unroll
+        for (int j = 1; j < BS_NV; j++) x = bmin2_nan(x, bmin2_nan(bmin2_nan(r[j].x, r[j].y), bmin2_nan(r[j].z, r[j].w)));
+        return fmin_nan(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    } else {
+        float m = __uint_as_float(r[0].x);
+#pragma unroll
+        for (int j = 0; j < BS_NV; j++)
+            m = fmin3_nan(fmin3_nan(m, __uint_as_float(r[j].x), __uint_as_float(r[j].y)), __uint_as_float(r[j].z),
+                          __uint_as_float(r[j].w));
+        return m;
+    }
+}
+
+// The same of the logits that are not masked (-inf and +inf for none).
+template <int DT>
+__device__ __forceinline__ void lane_extremes_open(const uint4 (&r)[BS_NV], float &mx, float &mn)
 {
     using T = DtypeTraits<DT>;
-    float mx, mn;
-    if constexpr (DT == G4S_BF16) {
-        uint32_t x = r[0].x, y = x;
+    mx = -__uint_as_float(0x7f800000u);
+    mn = -mx;
 #pragma unroll
-        for (int j = 0; j < BNV; j++) {
-            x = bmax2_nan(x, bmax2_nan(bmax2_nan(r[j].x, r[j].y), bmax2_nan(r[j].z, r[j].w)));
-            y = bmin2_nan(y, bmin2_nan(bmin2_nan(r[j].x, r[j].y), bmin2_nan(r[j].z, r[j].w)));
-        }
-        mx = fmax_nan(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-        mn = fmin_nan(__uint_as_float(y << 16), __uint_as_float(y & 0xffff0000u));
-    } else {
-        mx = mn = __uint_as_float(r[0].x);
-#pragma unroll
-        for (int j = 0; j < BNV; j++) {
-            mx = fmax3_nan(fmax3_nan(mx, __uint_as_float(r[j].x), __uint_as_float(r[j].y)), __uint_as_float(r[j].z),
-                           __uint_as_float(r[j].w));
-            mn = fmin3_nan(fmin3_nan(mn, __uint_as_float(r[j].x), __uint_as_float(r[j].y)), __uint_as_float(r[j].z),
-                           __uint_as_float(r[j].w));
-        }
-    }
-    const float lim = CAP ? fminf(a.softcap, 1e30f) : 3.402823466e38f;
-    const bool ok = mx <= lim && mn > (CAP ? -lim : -1e30f);  // a NaN fails both
-    if (!__all_sync(FULLMASK, ok)) return false;
-    u.m = warp_max_redux(mx);
-    u.c = beam_soft<CAP>(u.m, a);
-    const float2 ic = make_float2(a.invcap, a.invcap);
-    const float2 cap2 = make_float2(a.softcap, a.softcap);
-    const float2 nc = make_float2(-u.c, -u.c), k2 = make_float2(a.k, a.k);
-    float2 acc0 = make_float2(0.0f, 0.0f), acc1 = acc0;
-#pragma unroll
-    for (int j = 0; j < BNV; j++) {
+    for (int j = 0; j < BS_NV; j++) {
         float x[T::VW];
         T::unpack(r[j], x);
 #pragma unroll
-        for (int k = 0; k < T::VW; k += 2) {
-            const float2 v = make_float2(x[k], x[k + 1]);
-            float2 d;
-            if constexpr (CAP) d = __ffma2_rn(tanh_poly2(__fmul2_rn(v, ic)), cap2, nc);
-            else d = __fadd2_rn(v, nc);
-            const float2 y = __fmul2_rn(d, k2);
-            const float2 e = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-            if ((k >> 1) & 1) acc1 = __fadd2_rn(acc1, e);
-            else acc0 = __fadd2_rn(acc0, e);
+        for (int i = 0; i < T::VW; i++) {
+            const bool open = x[i] > -1e30f;
+            mx = open ? fmaxf(mx, x[i]) : mx;
+            mn = open ? fminf(mn, x[i]) : mn;
         }
     }
-    acc0 = __fadd2_rn(acc0, acc1);
-    float s = acc0.x + acc0.y;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(FULLMASK, s, d);
-    u.S = s;
-    return true;
 }
 
-// A beam that continues: a finite or infinite score (not -inf, not NaN) and not ended.
+// Adds 2^(s_i k - ref) (without softcap 2^((l_i - ref) k): the difference first, so that
+// k's rounding acts on the distance only) of a load to the lane's sums.  With the softcap
+// s k = l H(l^2), H a polynomial of NH coefficients with k and the cap folded in.  MASKED:
+// some logits add nothing.
+template <int DT, int NH, bool MASKED>
+__device__ __forceinline__ void load_sum(const uint4 (&r)[BS_NV], const uint64_t *h, uint64_t k, float ref, uint64_t &s0, uint64_t &s1)
+{
+    using T = DtypeTraits<DT>;
+    const uint64_t nref = two(-ref, -ref);
+#pragma unroll
+    for (int j = 0; j < BS_NV; j++) {
+        float x[T::VW];
+        T::unpack(r[j], x);
+#pragma unroll
+        for (int i = 0; i < T::VW; i += 2) {
+            const uint64_t v = two(x[i], x[i + 1]);
+            uint64_t y;
+            if constexpr (NH > 0) {
+                const uint64_t q = mul2(v, v);
+                uint64_t p = h[NH - 1];
+#pragma unroll
+                for (int c = NH - 2; c >= 0; c--) p = fma2(p, q, h[c]);
+                y = fma2(v, p, nref);
+            } else {
+                y = mul2(add2(v, nref), k);
+            }
+            const float2 z = halves(y);
+            float e0 = ex2_approx(z.x), e1 = ex2_approx(z.y);
+            if (MASKED) {
+                e0 = x[i] > -1e30f ? e0 : 0.0f;
+                e1 = x[i + 1] > -1e30f ? e1 : 0.0f;
+            }
+            const uint64_t e = two(e0, e1);
+            if ((i >> 1) & 1) s1 = add2(s1, e);
+            else s0 = add2(s0, e);
+        }
+    }
+}
+
+// A beam that continues: a score that is not -inf (nor NaN), and not ended.
 __device__ __forceinline__ bool beam_live(const BeamArgs &a, int row)
 {
     return a.scores[row] > -__uint_as_float(0x7f800000u) && !(a.done && a.done[row]);
 }
 
-// Persistent warps over the live rows' items; a unit's vectors are loaded while the
-// one before is reduced.
+// Persistent warps over the live rows' items; each lane copies its own vectors of the two
+// loads ahead into the warp's ring (cp.async: no registers, no barrier).  The ways through
+// a load:
+//   0  no logit above cap / 2: the polynomial of 5 coefficients (7 packed operations a
+//      pair).  Below -cap / 2 it falls faster than tanh, to -inf for masked logits (its
+//      last coefficient is positive); with the load's maximum at or above 0 and cap >=
+//      28 T what is lost there is under 1e-8 of the sum, so the smallest logit is not
+//      looked for; else it has to be at or above -cap / 2
+//   1  |l| <= cap: the polynomial of 8 coefficients
+//   2  the same with masked logits
+//   3  element by element: |l| > cap, a NaN, a row's ragged end
+// Without softcap way 0 takes all but NaNs and ends: 2^-inf is 0.
 template <int DT, bool VEC, bool CAP>
-__global__ void __launch_bounds__(BS_THREADS) beam_stream_kernel(const BeamArgs a)
+__global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const __grid_constant__ BeamArgs a)
 {
     using T = DtypeTraits<DT>;
-    constexpr int UNIT = BeamGeo<DT>::UNIT;
+    constexpr int LOAD = 32 * BS_NV * T::VW;  // logits of a load
     const float NEG_INF = -__uint_as_float(0x7f800000u);
+    __shared__ uint4 s_ring[VEC ? BS_THREADS / 32 * BS_STAGES * BS_NV * 32 : 1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
-    const int nw = (int)gridDim.x * (BS_THREADS / 32);
-    const int it0 = (int)blockIdx.x * (BS_THREADS / 32) + (threadIdx.x >> 5);
-    const int step_row = nw / a.ipr, step_sub = nw % a.ipr;
-    struct Cursor {
-        int row, item, u;  // u: unit within the item
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring + (VEC ? (threadIdx.x >> 5) * (BS_STAGES * BS_NV * 32) + lane : 0));
+    const int nw = (int)gridDim.x * (BS_THREADS / 32), w0 = (int)blockIdx.x * (BS_THREADS / 32) + (threadIdx.x >> 5);
+    const int step_row = nw / a.ipr, step_item = nw % a.ipr, item_len = a.upi * BeamGeo<DT>::UNIT;
+    struct Load {
+        int row, item, left;  // left: logits from its start to the item's end
+        const char *p;
     };
-    const int upr = (a.vocab + UNIT - 1) / UNIT;
-    auto skip_dead = [&](Cursor &c) {
-        while (c.row < a.rows && !beam_live(a, c.row)) {
-            c.item += step_sub;
-            c.row += step_row;
-            if (c.item >= a.ipr) {
-                c.item -= a.ipr;
-                c.row++;
+    auto find = [&](int row, int item) {  // the first live item from here on in the warp's steps
+        for (;; row += step_row, item += step_item) {
+            if (item >= a.ipr) {
+                item -= a.ipr;
+                row++;
             }
+            if (row >= a.rows) return Load{row, item, 0, nullptr};
+            if (beam_live(a, row)) break;
         }
+        const int e0 = item * item_len;
+        return Load{row, item, min(a.vocab - e0, item_len),
+                    (const char *)a.logits + ((int64_t)row * a.row_stride + e0) * T::ESIZE + (VEC ? lane * 16 : 0)};
     };
-    auto next = [&](Cursor c) {
-        if (c.u + 1 < a.upi && c.item * a.upi + c.u + 1 < upr) {
-            c.u++;
-            return c;
-        }
-        c.u = 0;
-        c.item += step_sub;
-        c.row += step_row;
-        if (c.item >= a.ipr) {
-            c.item -= a.ipr;
-            c.row++;
-        }
-        skip_dead(c);
-        return c;
+    auto after = [&](const Load &u) {
+        if (u.left > LOAD) return Load{u.row, u.item, u.left - LOAD, u.p + LOAD * T::ESIZE};
+        return u.row < a.rows ? find(u.row + step_row, u.item + step_item) : u;
     };
-    auto at = [&](const Cursor &c) {
-        return (const char *)a.logits +
-               ((int64_t)c.row * a.row_stride + (int64_t)(c.item * a.upi + c.u) * UNIT) * T::ESIZE;
-    };
-    auto left = [&](const Cursor &c) { return a.vocab - (c.item * a.upi + c.u) * UNIT; };
-    Cursor cur{it0 / a.ipr, it0 % a.ipr, 0};
-    skip_dead(cur);
-    uint4 r[BNV] = {};
-    if (cur.row < a.rows && left(cur) >= UNIT) load_unit<DT, VEC>(at(cur), lane, r);
-    UnitStat acc{NEG_INF, 0.0f, 0.0f};
-    while (cur.row < a.rows) {
-        const Cursor nx = next(cur);
-        uint4 rn[BNV] = {};
-        if (nx.row < a.rows && left(nx) >= UNIT) load_unit<DT, VEC>(at(nx), lane, rn);
-        UnitStat u;
-        const int n = min(UNIT, left(cur));
-        if (n < UNIT || !unit_fast<DT, CAP>(r, a, u)) u = unit_general<DT, CAP>(at(cur), n, lane, a);
-        if (cur.u == 0) {
-            acc = u;
-        } else if (u.m > NEG_INF) {
-            if (u.m > acc.m) {
-                u.S += acc.m > NEG_INF ? acc.S * ex2_approx((acc.c - u.c) * a.k) : 0.0f;
-                acc = u;
-            } else {
-                acc.S += u.S * ex2_approx((u.c - acc.c) * a.k);
-            }
-        }
-        if (nx.u == 0 && lane == 0)
-            a.istat[(int64_t)cur.row * a.ipr + cur.item] = make_float4(acc.m, acc.c, acc.S, 0.0f);
-        cur = nx;
+    auto fetch = [&](const Load &u, uint32_t to) {
+        if (VEC && u.left >= LOAD) {
 #pragma unroll
-        for (int j = 0; j < BNV; j++) r[j] = rn[j];
+            for (int j = 0; j < BS_NV; j++)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + j * 512), "l"(u.p + j * 512) : "memory");
+        }
+        cp_async_commit();
+    };
+    uint64_t h1[BEAM_H1], k2 = two(a.k);
+#pragma unroll
+    for (int i = 0; i < BEAM_H1; i++) h1[i] = CAP ? two(a.h1[i]) : 0;
+    Load cur = find(w0 / a.ipr, w0 % a.ipr), nx = after(cur);
+    float m = NEG_INF, ref = 0.0f;
+    uint64_t s0 = 0, s1 = 0;
+    uint32_t at = ring;
+    fetch(cur, ring);
+    fetch(nx, ring + BS_NV * 512);
+    while (cur.row < a.rows) {
+        uint4 r[BS_NV];
+        const bool whole = cur.left >= LOAD, last = cur.left <= LOAD;
+        if constexpr (VEC) {
+            cp_async_wait<1>();
+#pragma unroll
+            for (int j = 0; j < BS_NV; j++)
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(r[j].x), "=r"(r[j].y), "=r"(r[j].z), "=r"(r[j].w)
+                             : "r"(at + j * 512) : "memory");
+        } else if (whole) {
+            load_unit<DT, false>(cur.p, lane, r);
+        }
+        float mx = NEG_INF;
+        int way = 3;
+        if (whole) {
+            mx = lane_max<DT>(r);  // (the loads from the ring are done: it can be refilled)
+            way = __all_sync(FULLMASK, CAP ? mx <= a.lim1 : mx <= beam_max<DT>()) ? 0 : 1;  // a NaN fails
+        }
+        const Load n2 = after(nx);
+        fetch(n2, at);
+        if (!whole || (way == 1 && !CAP)) {
+            way = 3;
+        } else if (CAP && (way == 1 || !(a.skip_min && __any_sync(FULLMASK, mx >= 0.0f)))) {
+            float mn = lane_min<DT>(r);
+            if (way == 1 || !__all_sync(FULLMASK, mn >= -a.lim1)) {
+                way = __all_sync(FULLMASK, mx <= a.lim2 && mn >= -a.lim2) ? 1 : 3;
+                if (way == 3) {
+                    lane_extremes_open<DT>(r, mx, mn);
+                    if (__all_sync(FULLMASK, mx <= a.lim2 && mn >= -a.lim2)) way = 2;
+                }
+            }
+        }
+        const char *p = cur.p - (VEC ? lane * 16 : 0);
+        const int n = min(cur.left, LOAD);
+        if (way == 3) {
+            mx = NEG_INF;
+#pragma unroll 4
+            for (int i = lane; i < n; i += 32) mx = fmaxf(mx, beam_raw<DT>(T::load1(p, i)));
+        }
+        mx = warp_max_redux(mx);
+        if (mx > -1e30f) {
+            // a new maximum moves the reference
+            if (mx > m) {
+                const float to = CAP ? __fmul_rn(beam_soft<CAP>(mx, a), a.k) : mx;
+                const float f = m > NEG_INF ? ex2_approx(CAP ? ref - to : (ref - to) * a.k) : 0.0f;
+                s0 = mul2(s0, two(f, f));
+                s1 = mul2(s1, two(f, f));
+                m = mx;
+                ref = to;
+            }
+            if (way == 0) {
+                load_sum<DT, CAP ? BEAM_H1 : 0, false>(r, h1, k2, ref, s0, s1);
+            } else if (CAP && way < 3) {
+                uint64_t h2[BEAM_H2];
+#pragma unroll
+                for (int i = 0; i < BEAM_H2; i++) h2[i] = two(a.h2[i]);
+                if (way == 1) load_sum<DT, CAP ? BEAM_H2 : 0, false>(r, h2, k2, ref, s0, s1);
+                else load_sum<DT, CAP ? BEAM_H2 : 0, true>(r, h2, k2, ref, s0, s1);
+            } else {
+                float s = 0.0f;
+#pragma unroll 4
+                for (int i = lane; i < n; i += 32) {
+                    const float v = beam_raw<DT>(T::load1(p, i));
+                    const float e = ex2_approx(CAP ? __fmaf_rn(beam_soft<CAP>(v, a), a.k, -ref) : (v - ref) * a.k);
+                    s += v == NEG_INF ? 0.0f : e;
+                }
+                s0 = add2(s0, two(s, 0.0f));
+            }
+        }
+        if (last) {
+            const float2 x = halves(add2(s0, s1));
+            float S = x.x + x.y;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(FULLMASK, S, d);
+            if (lane == 0) a.istat[(int64_t)cur.row * a.ipr + cur.item] = make_float4(m, ref, S, 0.0f);
+            m = NEG_INF;
+            ref = 0.0f;
+            s0 = s1 = 0;
+        }
+        cur = nx;
+        nx = n2;
+        at = at == ring ? ring + BS_NV * 512 : ring;
     }
+    cp_async_wait<0>();
 }
 
 // ---------------------------------------------------------------------------
 // combine
 // ---------------------------------------------------------------------------
-struct BeamRow {
-    double ln, inv;  // log of the row's sum (in units of c), 1 / max(length, 1)^alpha
-    float score, c;
-    int len, kind;   // kind: BEAM_DEAD, BEAM_LIVE, BEAM_DONE
+// What is needed to more than 32 bits (the beams' scores meet here) is a sum of two fp32
+// numbers, high + low.  Measured on this GPU, one dependent 64-bit operation takes about
+// 48 cycles and 128 scores in 64 bits 9000; the routines below are exact to 3e-11 of
+// their result (checked against 80 bits over their ranges).
+struct Pair {
+    float h, l;
 };
-enum { BEAM_DEAD = 0, BEAM_LIVE = 1, BEAM_DONE = 2 };
-
-__device__ __forceinline__ double beam_score(const BeamArgs &a, const BeamRow &r, uint32_t key)
+__device__ __forceinline__ Pair pair_sum(float a, float b)  // a + b, exactly
 {
-    if (r.kind == BEAM_DONE) return (double)r.score;
-    double s = (double)key2f(key);
-    if (a.softcap > 0.0f) s = (double)a.softcap * tanh(s / (double)a.softcap);
-    return (double)r.score + ((s - (double)r.c) / a.temperature - r.ln);
+    const float s = __fadd_rn(a, b), bb = __fsub_rn(s, a);
+    return {s, __fadd_rn(__fsub_rn(a, __fsub_rn(s, bb)), __fsub_rn(b, bb))};
 }
+__device__ __forceinline__ Pair pair_norm(float a, float b)  // a + b, exactly, for |a| >= |b|
+{
+    const float s = __fadd_rn(a, b);
+    return {s, __fsub_rn(b, __fsub_rn(s, a))};
+}
+__device__ __forceinline__ Pair pair_add(Pair a, Pair b)
+{
+    const Pair s = pair_sum(a.h, b.h);
+    return pair_norm(s.h, __fadd_rn(s.l, __fadd_rn(a.l, b.l)));
+}
+__device__ __forceinline__ Pair pair_mul(Pair a, Pair b)
+{
+    const float p = __fmul_rn(a.h, b.h);
+    return pair_norm(p, __fmaf_rn(a.h, b.l, __fmaf_rn(a.l, b.h, __fmaf_rn(a.h, b.h, -p))));
+}
+
+// e^z for -80 <= z <= 80: z = n ln2 / 4 + f, |f| <= ln2 / 8, the Taylor series to f^6 (its
+// first terms as pairs), times 2^(n / 4).
+static __device__ __noinline__ Pair pair_exp(Pair z)
+{
+    const float t = rintf(__fmul_rn(z.h, 5.770780087f));
+    const int n = (int)t;
+    // ln2 / 4 in 15 bits, so that the first difference is exact, and the rest
+    const Pair f = pair_sum(__fmaf_rn(t, -0.17328643798828125f, z.h), __fmaf_rn(t, -3.571516913e-07f, z.l));
+    const float g = __fmul_rn(f.h, f.h), gl = __fmaf_rn(f.h, f.h, -g);
+    float c = __fmaf_rn(f.h, 1.0f / 720.0f, 1.0f / 120.0f);
+    c = __fmaf_rn(f.h, c, 1.0f / 24.0f);
+    c = __fmaf_rn(f.h, c, 1.0f / 6.0f);
+    const float cubic = __fmul_rn(__fmul_rn(f.h, g), c);
+    Pair s = pair_sum(f.h, 0.5f * g);
+    s = pair_norm(s.h, __fadd_rn(__fadd_rn(s.l, f.l), __fadd_rn(__fmaf_rn(0.5f, gl, __fmul_rn(f.h, f.l)), cubic)));
+    const Pair o = pair_sum(1.0f, s.h);
+    const Pair e = pair_norm(o.h, __fadd_rn(o.l, s.l));
+    const int q = n & 3;
+    const Pair root = q < 2 ? (q ? Pair{1.189207077f, 3.797635273e-08f} : Pair{1.0f, 0.0f})
+                            : (q == 2 ? Pair{1.414213538f, 2.420323497e-08f} : Pair{1.681792855f, -2.475532668e-08f});
+    const Pair v = pair_mul(e, root);
+    const float scale = pow2i(n >> 2);
+    return {v.h * scale, v.l * scale};
+}
+
+// log s for 2^-60 <= s <= 2^60: a first value by the hardware, then ln(s e^-y) from its
+// difference to 1.
+__device__ __forceinline__ Pair pair_log(Pair s)
+{
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(s.h));
+    y *= 0.693147181f;
+    const Pair u = pair_mul(s, pair_exp(Pair{-y, 0.0f}));
+    const float d = __fadd_rn(__fsub_rn(u.h, 1.0f), u.l);
+    return pair_norm(y, __fmaf_rn(-0.5f * d, d, d));
+}
+
+enum { BEAM_DEAD = 0, BEAM_LIVE = 1, BEAM_DONE = 2 };
+struct BeamRow {
+    Pair base, inv;  // score less log of the row's sum (with the softcap less ref too); 1 / max(length, 1)^alpha
+    float score, ref;
+    int len, kind;
+};
+
+// What a logit adds to its row's base: cap tanh(l / cap) / T, tanh(q) = 1 - 2 / (e^2q + 1)
+// (its cancellation for small q costs 3e-11 of the cap), or (l - ref) / T.
+__device__ __forceinline__ Pair beam_x(const BeamArgs &a, float ref, uint32_t key)
+{
+    const float l = key2f(key);
+    if (a.softcap > 0.0f) {
+        const float b = 2.0f * fminf(fabsf(l), 20.0f * a.softcap);  // beyond, tanh is 1 to 2^-57
+        Pair z;
+        z.h = __fmul_rn(b, a.invcap2[0]);
+        z.l = __fmaf_rn(b, a.invcap2[1], __fmaf_rn(b, a.invcap2[0], -z.h));
+        const Pair e = pair_exp(z);
+        Pair d = pair_sum(e.h, 1.0f);
+        d.l = __fadd_rn(d.l, e.l);
+        const float w = __frcp_rn(d.h), off = __fsub_rn(__fmaf_rn(-d.h, w, 1.0f), __fmul_rn(d.l, w));
+        const Pair th = pair_sum(1.0f, -2.0f * w);
+        const Pair x = pair_mul(pair_norm(th.h, __fsub_rn(th.l, 2.0f * w * off)), Pair{a.scale2[0], a.scale2[1]});
+        return l < 0.0f ? Pair{-x.h, -x.l} : x;
+    }
+    const Pair d = pair_sum(l, -ref);
+    const float x = __fmul_rn(d.h, a.scale2[0]);
+    // far below any other, perhaps -inf
+    return fabsf(d.h) < 1e30f && fabsf(x) < 1e30f ? pair_mul(d, Pair{a.scale2[0], a.scale2[1]}) : Pair{x, 0.0f};
+}
+
+// A continuation's score from its x.
+__device__ __forceinline__ Pair beam_score(const BeamRow &r, Pair x)
+{
+    if (r.kind == BEAM_DONE) return {r.score, 0.0f};
+    return fabsf(x.h) < 1e30f ? pair_add(r.base, x) : x;
+}
+
+// A pair as a whole number that orders as it does, and its bits.
+__device__ __forceinline__ uint64_t beam_rank(const BeamRow &r, Pair score, bool scaled)
+{
+    if (scaled && fabsf(score.h) < 1e30f) score = pair_mul(score, r.inv);
+    return ((uint64_t)f2key(score.h + 0.0f) << 32) | f2key(score.l + 0.0f);
+}
+__device__ __forceinline__ uint64_t pair_bits(Pair x) { return ((uint64_t)__float_as_uint(x.h) << 32) | __float_as_uint(x.l); }
+__device__ __forceinline__ Pair bits_pair(uint64_t b) { return {__uint_as_float((uint32_t)(b >> 32)), __uint_as_float((uint32_t)b)}; }
 
 // Order of two continuations: rank, then the lower beam, the larger raw logit, the lower
 // id (item): the latter three in one number, larger first.
@@ -288,314 +515,352 @@ __device__ __forceinline__ int tie_beam(uint64_t t) { return 255 - (int)(t >> 56
 __device__ __forceinline__ uint32_t tie_key(uint64_t t) { return (uint32_t)(t >> 24); }
 __device__ __forceinline__ uint32_t tie_id(uint64_t t) { return 0xffffffu - (uint32_t)(t & 0xffffffu); }
 
-// Sorts P (a power of two) pairs in shared memory, first in order first.
-__device__ __forceinline__ void beam_sort(double *rank, uint64_t *tie, int P)
+__device__ __forceinline__ bool beam_before(const ulonglong2 &x, const ulonglong2 &y)
 {
-    for (int k = 2; k <= P; k <<= 1) {
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int t = threadIdx.x; t < P / 2; t += BC_THREADS) {
-                const int i = 2 * t - (t & (j - 1)), o = i + j;
-                const double ri = rank[i], ro = rank[o];
-                const uint64_t ti = tie[i], to = tie[o];
-                const bool o_first = ro > ri || (ro == ri && to > ti);
-                if (o_first == ((i & k) == 0)) {
-                    rank[i] = ro;
-                    rank[o] = ri;
-                    tie[i] = to;
-                    tie[o] = ti;
-                }
-            }
-            __syncthreads();
-        }
-    }
+    return (x.x > y.x) | ((x.x == y.x) & (x.y > y.y));  // (no branch)
 }
 
-// The keys of unit u of an item (0: masked or past the row).
+// The first N of n entries (rank, tie) in shared memory, in order, to out; rest(tie) for
+// each of the others.  Up to 512 entries every one counts those before it, a warp four
+// entries at a time; more are sorted in place (padded with zeros to P, a power of two).
+// Pairs closer than 64 places stay within a warp's 32 exchanges, so only the wider steps
+// need the CTA.
+template <class Rest>
+__device__ __forceinline__ void beam_first(ulonglong2 *v, int n, int P, int N, ulonglong2 *out, Rest rest)
+{
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (n <= 512) {
+        for (int e0 = tid / 32 * 4; e0 < n; e0 += BC_WARPS * 4) {
+            ulonglong2 x[4];
+            int before[4] = {};
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = v[e0 + k];  // (zeros from n on)
+            for (int i = lane; i < n; i += 32) {
+                const ulonglong2 y = v[i];
+#pragma unroll
+                for (int k = 0; k < 4; k++) before[k] += beam_before(y, x[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int c = __reduce_add_sync(FULLMASK, before[k]);
+                if (x[k].y && lane == k) {
+                    if (c < N) out[c] = x[k];
+                    else rest(x[k].y);
+                }
+            }
+        }
+    } else {
+        for (int k = 2; k <= P; k <<= 1) {
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                for (int t = tid; t < P / 2; t += BC_THREADS) {
+                    const int i = 2 * t - (t & (j - 1)), o = i + j;
+                    const ulonglong2 x = v[i], y = v[o];
+                    if (beam_before(y, x) == ((i & k) == 0)) {
+                        v[i] = y;
+                        v[o] = x;
+                    }
+                }
+                const int jn = j > 1 ? j >> 1 : k;  // the next step's distance
+                if (j > 32 || jn > 32) __syncthreads();
+                else __syncwarp();
+            }
+        }
+        __syncthreads();
+        for (int e = tid; e < n; e += BC_THREADS) {
+            if (v[e].y == 0) continue;
+            if (e < N) out[e] = v[e];
+            else rest(v[e].y);
+        }
+    }
+    __syncthreads();
+}
+
+// The smallest logit with at least this key (NaN, which no logit reaches, above the
+// largest finite one's, which +inf has too).
+template <int DT>
+__device__ __forceinline__ float beam_floor(uint32_t key)
+{
+    return key > f2key(beam_max<DT>()) ? __uint_as_float(0x7fc00000u) : key2f(key);
+}
+constexpr uint32_t BEAM_KEY_MIN = 0xeb60d36u;  // the key after -1e30's
+
+// Which of the lane's logits of a unit (n left) are at or above x: bit j * VW + k for
+// logit (j, k).
 template <int DT, bool VEC>
-__device__ __forceinline__ void unit_keys(const char *p, int n, int lane, uint32_t (&key)[BeamGeo<DT>::EPL])
+__device__ __forceinline__ uint32_t unit_mask(const char *p, int n, int lane, float x)
 {
     using T = DtypeTraits<DT>;
-    if (n >= BeamGeo<DT>::UNIT) {
+    uint32_t m = 0;
+    if (VEC && n >= BeamGeo<DT>::UNIT) {
         uint4 r[BNV];
-        load_unit<DT, VEC>(p, lane, r);
+#pragma unroll
+        for (int j = 0; j < BNV; j++) r[j] = __ldg((const uint4 *)p + j * 32 + lane);
 #pragma unroll
         for (int j = 0; j < BNV; j++) {
-            float x[T::VW];
-            T::unpack(r[j], x);
+            float v[T::VW];
+            T::unpack(r[j], v);
 #pragma unroll
-            for (int k = 0; k < T::VW; k++) key[j * T::VW + k] = beam_key(x[k]);
+            for (int k = 0; k < T::VW; k++) m |= (v[k] >= x ? 1u : 0u) << (j * T::VW + k);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < BNV; j++)
-#pragma unroll
-            for (int k = 0; k < T::VW; k++) {
-                const int e = (j * 32 + lane) * T::VW + k;
-                key[j * T::VW + k] = e < n ? beam_key(T::load1(p, e)) : 0u;
-            }
+        for (int i = 0; i < BeamGeo<DT>::EPL; i++) {
+            const int e = ((i / T::VW) * 32 + lane) * T::VW + i % T::VW;
+            if (e < n && T::load1(p, e) >= x) m |= 1u << i;
+        }
     }
+    return m;
 }
 
 template <int DT, bool VEC>
-__global__ void __launch_bounds__(BC_THREADS) beam_combine_kernel(const BeamArgs a)
+__global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __grid_constant__ BeamArgs a)
 {
     using T = DtypeTraits<DT>;
-    constexpr int UNIT = BeamGeo<DT>::UNIT, EPL = BeamGeo<DT>::EPL;
-    const double NEG_INF = -__longlong_as_double(0x7ff0000000000000ll);
-    extern __shared__ double s_mem[];
-    double *e_rank = s_mem;                              // [pe] the beams' items
-    uint64_t *e_tie = (uint64_t *)(e_rank + a.pe);
-    double *c_rank = (double *)(e_tie + a.pe);           // [pc] collected tokens
-    uint64_t *c_tie = (uint64_t *)(c_rank + a.pc);
+    constexpr int UNIT = BeamGeo<DT>::UNIT, SH = DT == G4S_BF16 ? 16 : 0;
+    const float NEG_INF = -__uint_as_float(0x7f800000u);
+    extern __shared__ ulonglong2 s_mem[];
+    ulonglong2 *ent = s_mem;                         // [pe] the beams' items: (rank, tie), rank 0: none
+    ulonglong2 *cand = ent + a.pe;                   // [pc] collected tokens
+    ulonglong2 *first = cand + a.pc;                 // [n_out] the first in order
     __shared__ BeamRow s_row[G4S_BEAM_MAX];
-    __shared__ int s_cnt[G4S_BEAM_MAX], s_sel[G4S_BEAM_MAX];
-    __shared__ unsigned long long s_thr[G4S_BEAM_MAX];
+    __shared__ int s_sel[G4S_BEAM_MAX];      // items of the row among the first
+    __shared__ uint32_t s_least[G4S_BEAM_MAX];  // the least key of its tokens wanted
     __shared__ int s_m;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int W = a.beams, N = a.n_out, row0 = (int)blockIdx.x * W;
 
-    for (int e = tid; e < a.pe; e += BC_THREADS) {
-        e_rank[e] = NEG_INF;
-        e_tie[e] = 0;
-    }
-    for (int e = tid; e < a.pc; e += BC_THREADS) {
-        c_rank[e] = NEG_INF;
-        c_tie[e] = 0;
-    }
+    for (int e = tid; e < a.pe + a.pc + N; e += BC_THREADS) s_mem[e] = make_ulonglong2(0, 0);
     if (tid < G4S_BEAM_MAX) {
-        s_thr[tid] = 0;
+        s_least[tid] = BEAM_KEY_MIN;
         s_sel[tid] = 0;
-        s_cnt[tid] = 0;
     }
     if (tid == 0) s_m = 0;
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // 1. a warp a beam: the row's sum, its n_out largest items
-    for (int w = warp; w < W; w += BC_WARPS) {
-        const int row = row0 + w;
-        BeamRow r;
-        r.score = a.scores[row];
-        r.len = a.lens ? a.lens[row] : 0;
-        r.kind = !(r.score > -__uint_as_float(0x7f800000u)) ? BEAM_DEAD : (a.done && a.done[row]) ? BEAM_DONE : BEAM_LIVE;
-        r.c = 0.0f;
-        r.ln = 0.0;
-        const int length = r.kind == BEAM_LIVE ? r.len + 1 : r.len;
-        r.inv = a.alpha == 0.0 ? 1.0 : pow((double)max(length, 1), -a.alpha);
-        int cnt = 0;
-        if (r.kind == BEAM_DONE) {
-            cnt = 1;
-            if (lane == 0) e_tie[w * N] = beam_tie(w, 0u, 0u);
-        } else if (r.kind == BEAM_LIVE) {
-            const float4 *st = a.istat + (int64_t)row * a.ipr;
-            uint32_t key[BIPL];
-            float c = -__uint_as_float(0x7f800000u);
-            uint32_t kmax = 0;
+    // 1. two warps a beam: one sums the row, the other takes its n_out largest items
+    for (int task = warp; task < 2 * W; task += BC_WARPS) {
+        const bool sums = task < W;
+        const int w = sums ? task : task - W, row = row0 + w;
+        const float4 *st = a.istat + (int64_t)row * a.ipr;
+        float4 q[BIPL];  // (a dead row's are what an earlier call left, and are not used)
+#pragma unroll
+        for (int j = 0; j < BIPL; j++)
+            q[j] = j * 32 + lane < a.ipr ? __ldcg(st + j * 32 + lane) : make_float4(NEG_INF, NEG_INF, 0.0f, 0.0f);
+        const float score = a.scores[row];
+        const int len = a.lens ? a.lens[row] : 0;
+        const int kind = !(score > NEG_INF) ? BEAM_DEAD : (a.done && a.done[row]) ? BEAM_DONE : BEAM_LIVE;
+        uint32_t key[BIPL], kmax = 0;  // (bf16 keys: the upper half tells them apart)
+#pragma unroll
+        for (int j = 0; j < BIPL; j++) {
+            key[j] = beam_key<DT>(q[j].x) >> SH;
+            kmax = max(kmax, key[j]);
+        }
+        const uint32_t best = __reduce_max_sync(FULLMASK, kmax);
+        const bool live = kind == BEAM_LIVE && best;
+        if (sums) {
+            BeamRow r{{0.0f, 0.0f}, {1.0f, 0.0f}, score, 0.0f, len, kind};
+            if (live) {
+                float ref = NEG_INF;
+#pragma unroll
+                for (int j = 0; j < BIPL; j++)
+                    if (key[j]) ref = fmaxf(ref, q[j].y);
+                r.ref = warp_max_redux(ref);
+                Pair sum{0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < BIPL; j++) {
+                    const Pair s = pair_sum(sum.h, key[j] ? q[j].z * ex2_approx((q[j].y - r.ref) * a.ref32) : 0.0f);
+                    sum = {s.h, sum.l + s.l};
+                }
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) {
+                    const Pair s = pair_sum(sum.h, __shfl_xor_sync(FULLMASK, sum.h, d));
+                    sum = {s.h, s.l + (sum.l + __shfl_xor_sync(FULLMASK, sum.l, d))};
+                }
+                const Pair ln = pair_log(pair_norm(sum.h, sum.l));
+                r.base = pair_add(Pair{score, 0.0f}, Pair{-ln.h, -ln.l});
+                if (a.softcap > 0.0f)  // ref is in powers of two
+                    r.base = pair_add(r.base, pair_mul(Pair{-r.ref, 0.0f}, Pair{0.693147182f, -1.904654212e-09f}));
+            }
+            if (a.alpha2[0] != 0.0f) {
+                const int length = max(kind == BEAM_LIVE ? len + 1 : len, 1);
+                const Pair ln = pair_log(pair_sum((float)(length & 0xffff), (float)(length & 0x7fff0000)));
+                r.inv = pair_exp(pair_mul(ln, Pair{-a.alpha2[0], -a.alpha2[1]}));
+            }
+            if (lane == 0) s_row[w] = r;
+        } else if (kind == BEAM_DONE) {
+            if (lane == 0) ent[w * N].y = beam_tie(w, 0u, 0u);
+        } else if (live) {
+            auto full = [](uint32_t k) { return SH ? (k << SH) | (k & 0x8000u ? 0u : 0xffffu) : k; };
             int nv = 0;
 #pragma unroll
+            for (int j = 0; j < BIPL; j++) nv += __popc(__ballot_sync(FULLMASK, key[j] != 0));
+            // the largest `above` with at least N items at or above it, between the least of
+            // the lanes' largest (for N <= 32) and the largest; out early at N exactly
+            const int cnt = min(N, nv);
+            uint32_t above = 0;  // keys over it are taken, then those equal to it
+            if (nv > N) {
+                uint32_t lo = max(N <= 32 ? __reduce_min_sync(FULLMASK, kmax) : 0u, 1u), hi = best;
+                for (above = lo; lo < hi;) {
+                    const uint32_t mid = lo + (hi - lo + 1) / 2;
+                    int n = 0;
+#pragma unroll
+                    for (int j = 0; j < BIPL; j++) n += __popc(__ballot_sync(FULLMASK, key[j] >= mid));
+                    if (n == N) {
+                        above = mid - 1;
+                        break;
+                    }
+                    if (n > N) lo = mid;
+                    else hi = mid - 1;
+                    above = lo;
+                }
+            }
+            const unsigned below = (1u << lane) - 1;
+            int o = w * N;
+#pragma unroll
             for (int j = 0; j < BIPL; j++) {
-                const int i = j * 32 + lane;
-                key[j] = 0;
-                if (i < a.ipr) {
-                    const float4 q = __ldcg(st + i);
-                    key[j] = beam_key(q.x);
-                    if (key[j]) c = fmaxf(c, q.y);
-                }
-                kmax = max(kmax, key[j]);
-                nv += key[j] != 0;
+                const unsigned b = __ballot_sync(FULLMASK, key[j] > above);
+                if (key[j] > above) ent[o + __popc(b & below)].y = beam_tie(w, full(key[j]), (uint32_t)(j * 32 + lane));
+                o += __popc(b);
             }
-            const uint32_t kmin = __reduce_min_sync(FULLMASK, kmax);  // every lane holds an item at or above it
-            kmax = __reduce_max_sync(FULLMASK, kmax);
-            nv = __reduce_add_sync(FULLMASK, nv);
-            if (nv == 0) {
-                r.kind = BEAM_DEAD;
-            } else {
-                c = warp_max_redux(c);
-                double sum = 0.0;
+            if (o < w * N + cnt) {  // equals, the lowest first
 #pragma unroll
                 for (int j = 0; j < BIPL; j++) {
-                    if (key[j]) {
-                        const float4 q = __ldcg(st + j * 32 + lane);
-                        // 2^((c_i - c) k): whole and fractional part, the difference exact in 64 bits
-                        const double y = ((double)q.y - (double)c) * a.k64;
-                        const double whole = rint(fmax(y, -1000.0));
-                        sum += (double)q.z * (double)ex2_approx((float)(y - whole < -1.0 ? -1.0 : y - whole)) *
-                               __longlong_as_double((long long)(1023 + (int)whole) << 52);
-                    }
-                }
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(FULLMASK, sum, d);
-                r.c = c;
-                r.ln = log(sum);
-                // the largest thr with at least N items at or above it
-                cnt = min(N, nv);
-                uint32_t thr = 0;  // keys above thr are taken, then those equal to it
-                int eq = 0;
-                if (nv > N) {
-                    uint32_t lo = N <= 32 ? kmin : 0u, hi = kmax;  // count(>= lo) >= N
-                    if (lo == 0) lo = 1;
-                    bool exact = false;
-                    while (lo < hi) {
-                        const uint32_t mid = lo + (hi - lo + 1) / 2;
-                        int n = 0;
-#pragma unroll
-                        for (int j = 0; j < BIPL; j++) n += key[j] >= mid;
-                        n = __reduce_add_sync(FULLMASK, n);
-                        if (n == N) {
-                            thr = mid - 1;
-                            exact = true;
-                            break;
-                        }
-                        if (n > N) lo = mid;
-                        else hi = mid - 1;
-                    }
-                    if (!exact) {
-                        thr = lo;
-                        eq = 1;
-                    }
-                }
-                int base = w * N;
-#pragma unroll
-                for (int j = 0; j < BIPL; j++) {
-                    const bool take = key[j] > thr;
-                    const unsigned b = __ballot_sync(FULLMASK, take);
-                    if (take) e_tie[base + __popc(b & ((1u << lane) - 1))] = beam_tie(w, key[j], (uint32_t)(j * 32 + lane));
-                    base += __popc(b);
-                }
-                if (eq) {
-#pragma unroll
-                    for (int j = 0; j < BIPL; j++) {
-                        const bool take = key[j] == thr;
-                        const unsigned b = __ballot_sync(FULLMASK, take);
-                        const int o = base + __popc(b & ((1u << lane) - 1));
-                        if (take && o < w * N + cnt) e_tie[o] = beam_tie(w, key[j], (uint32_t)(j * 32 + lane));
-                        base += __popc(b);
-                    }
+                    const unsigned b = __ballot_sync(FULLMASK, key[j] == above);
+                    const int at = o + __popc(b & below);
+                    if (key[j] == above && at < w * N + cnt) ent[at].y = beam_tie(w, full(above), (uint32_t)(j * 32 + lane));
+                    o += __popc(b);
                 }
             }
-        }
-        if (lane == 0) {
-            s_row[w] = r;
-            s_cnt[w] = cnt;
+            __syncwarp();
+            const float ref = key2f(full(best));
+            for (int i = lane; i < cnt; i += 32) ent[w * N + i].x = pair_bits(beam_x(a, ref, tie_key(ent[w * N + i].y)));
         }
     }
     __syncthreads();
 
     // 2. the items by their best token
+    const bool scaled = a.alpha2[0] != 0.0f;
     for (int e = tid; e < W * N; e += BC_THREADS) {
-        const uint64_t t = e_tie[e];
-        if (t) {
-            const BeamRow &r = s_row[tie_beam(t)];
-            e_rank[e] = beam_score(a, r, tie_key(t)) * r.inv;
+        const ulonglong2 v = ent[e];
+        if (v.y) {
+            const BeamRow &r = s_row[tie_beam(v.y)];
+            ent[e].x = beam_rank(r, beam_score(r, bits_pair(v.x)), scaled);
         }
     }
     __syncthreads();
-    beam_sort(e_rank, e_tie, a.pe);
-    int total = 0;
-    for (int w = 0; w < W; w++) total += s_cnt[w];
-    const int nsel = min(N, total);
     // a beam's tokens count from its best item left out; where all of its N items are
     // in, from the last of them; where it has no more, all
-    for (int e = tid; e < total; e += BC_THREADS) {
-        const int w = tie_beam(e_tie[e]);
-        if (e < nsel) atomicAdd(&s_sel[w], 1);
-        else atomicMax(&s_thr[w], (unsigned long long)e_tie[e]);
+    beam_first(ent, W * N, a.pe, N, first, [&](uint64_t tie) { atomicMax(&s_least[tie_beam(tie)], tie_key(tie)); });
+    const bool chosen = tid < N && first[tid].y;
+    if (chosen) atomicAdd(&s_sel[tie_beam(first[tid].y)], 1);
+    const int nsel = __syncthreads_count(chosen);
+    if (tid == 0 && nsel == N) {
+        const uint64_t t = first[N - 1].y;
+        if (s_sel[tie_beam(t)] == N) s_least[tie_beam(t)] = max(tie_key(t), BEAM_KEY_MIN);
     }
-    __syncthreads();
-    if (tid == 0 && nsel == N && s_sel[tie_beam(e_tie[N - 1])] == N) s_thr[tie_beam(e_tie[N - 1])] = e_tie[N - 1] - 1;
     __syncthreads();
 
-    // 3. their tokens
-    for (int j = warp; j < nsel; j += BC_WARPS) {
-        const uint64_t t = e_tie[j];
-        const int w = tie_beam(t), quota = N - j;
+    // 3. their tokens, a warp a unit.  Where they are more than fit (equal logits, a small
+    // vocabulary), again item by item: only n_out - j of the item in place j can count (the
+    // j items before it hold a better token each).
+    auto push = [&](int w, uint32_t key, int64_t id) {
+        const int o = atomicAdd(&s_m, 1);
+        if (o < a.pc) cand[o] = make_ulonglong2(0, beam_tie(w, key, (uint32_t)id));
+    };
+    auto place = [&](int i) { return ((i / T::VW) * 32 + lane) * T::VW + i % T::VW; };
+    for (int task = warp; task < nsel * a.upi; task += BC_WARPS) {
+        const uint64_t t = first[task / a.upi].y;
+        const int w = tie_beam(t), u = task % a.upi;
         if (s_row[w].kind == BEAM_DONE) {
-            if (lane == 0) c_tie[atomicAdd(&s_m, 1)] = t;
+            if (lane == 0 && u == 0) push(w, 0u, 0);
             continue;
         }
-        const uint32_t item = tie_id(t);
-        const uint64_t thr = s_thr[w];
-        const int64_t e0 = (int64_t)item * a.upi * UNIT;
-        const int n = (int)min((int64_t)a.upi * UNIT, a.vocab - e0);
+        const int64_t e0 = ((int64_t)tie_id(t) * a.upi + u) * UNIT;
+        const int n = (int)min((int64_t)UNIT, a.vocab - e0);
+        if (n <= 0) continue;
         const char *p = (const char *)a.logits + ((int64_t)(row0 + w) * a.row_stride + e0) * T::ESIZE;
-        uint32_t first[EPL];  // the first unit's keys; 0: not wanted
-        auto want = [&](uint32_t key) { return key && beam_tie(w, key, item) > thr; };
-        auto load = [&](int u, uint32_t(&key)[EPL]) {
-            unit_keys<DT, VEC>(p + (int64_t)u * UNIT * T::ESIZE, n - u * UNIT, lane, key);
-#pragma unroll
-            for (int i = 0; i < EPL; i++)
-                if (!want(key[i])) key[i] = 0;
-        };
-        // each unit's keys and the position of the lane's first logit in the item
-        auto for_units = [&](auto &&f) {
-            f(first, 0);
-            for (int u = 1; u * UNIT < n; u++) {
-                uint32_t key[EPL];
-                load(u, key);
-                f(key, u * UNIT);
-            }
-        };
-        load(0, first);
-        auto pos = [&](int i) { return ((i / T::VW) * 32 + lane) * T::VW + i % T::VW; };
-        auto count = [&](uint32_t least) {  // wanted keys at or above `least`
-            int c = 0;
-            for_units([&](const uint32_t(&key)[EPL], int) {
-#pragma unroll
-                for (int i = 0; i < EPL; i++) c += key[i] >= least;
-            });
-            return (int)__reduce_add_sync(FULLMASK, c);
-        };
-        auto push = [&](uint32_t above, uint32_t equal, int last) {  // keys > above; == equal up to position `last`
-            for_units([&](const uint32_t(&key)[EPL], int at) {
-#pragma unroll
-                for (int i = 0; i < EPL; i++)
-                    if (key[i] > above || (equal && key[i] == equal && at + pos(i) <= last))
-                        c_tie[atomicAdd(&s_m, 1)] = beam_tie(w, key[i], (uint32_t)(e0 + at + pos(i)));
-            });
-        };
-        if (count(1u) <= quota) {
-            push(0u, 0u, 0);
-        } else {
-            // only quota of them can count (the j items before hold a better token each): the
-            // quota-th largest key, then the position up to which its equals are taken
-            uint32_t lo = 1u, hi = 0xffffffffu;
-            while (lo < hi) {
-                const uint32_t mid = lo + (hi - lo) / 2 + 1;
-                if (count(mid) >= quota) lo = mid;
-                else hi = mid - 1;
-            }
-            const int need = quota - (lo == 0xffffffffu ? 0 : count(lo + 1));
-            int p0 = 0, p1 = n - 1;
-            while (p0 < p1) {
-                const int mid = (p0 + p1) / 2;
-                int c = 0;
-                for_units([&](const uint32_t(&key)[EPL], int at) {
-#pragma unroll
-                    for (int i = 0; i < EPL; i++) c += key[i] == lo && at + pos(i) <= mid;
-                });
-                if ((int)__reduce_add_sync(FULLMASK, c) >= need) p1 = mid;
-                else p0 = mid + 1;
-            }
-            push(lo, lo, p0);
+        for (uint32_t m = unit_mask<DT, VEC>(p, n, lane, beam_floor<DT>(s_least[w])); m; m &= m - 1) {
+            const int e = place(__ffs(m) - 1);
+            push(w, beam_key<DT>(T::load1(p, e)), e0 + e);
         }
     }
     __syncthreads();
-    const int m = s_m;
-    for (int e = tid; e < m; e += BC_THREADS) {
-        const BeamRow &r = s_row[tie_beam(c_tie[e])];
-        c_rank[e] = beam_score(a, r, tie_key(c_tie[e])) * r.inv;
+    int m = s_m;
+    if (m > a.pc) {
+        __syncthreads();
+        for (int e = tid; e < a.pc; e += BC_THREADS) cand[e] = make_ulonglong2(0, 0);
+        if (tid == 0) s_m = 0;
+        __syncthreads();
+        for (int j = warp; j < nsel; j += BC_WARPS) {
+            const uint64_t t = first[j].y;
+            const int w = tie_beam(t), quota = N - j;
+            if (s_row[w].kind == BEAM_DONE) {
+                if (lane == 0) push(w, 0u, 0);
+                continue;
+            }
+            const int64_t e0 = (int64_t)tie_id(t) * a.upi * UNIT;
+            const int n = (int)min((int64_t)a.upi * UNIT, a.vocab - e0);
+            const char *p = (const char *)a.logits + ((int64_t)(row0 + w) * a.row_stride + e0) * T::ESIZE;
+            auto count = [&](uint32_t key, uint32_t but, int upto) {  // of keys key .. but - 1, at places up to `upto`
+                int c = 0;
+#pragma unroll 1
+                for (int u = 0; u < n; u += UNIT) {
+                    const char *pu = p + (int64_t)u * T::ESIZE;
+                    uint32_t m = unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(key));
+                    if (but) m &= ~unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(but));
+                    for (; upto < n && m; m &= m - 1) c += u + place(__ffs(m) - 1) <= upto;
+                    c += __popc(m);
+                }
+                return (int)__reduce_add_sync(FULLMASK, c);
+            };
+            // the quota-th largest key, and the place up to which its equals are taken
+            uint32_t lo = s_least[w], hi = tie_key(t);
+            int last = n;
+            if (count(lo, 0u, n) > quota) {
+                while (lo < hi) {
+                    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+                    if (count(mid, 0u, n) >= quota) lo = mid;
+                    else hi = mid - 1;
+                }
+                const int need = quota - count(lo + 1, 0u, n);
+                int p0 = 0;
+                last = n - 1;
+                while (p0 < last) {
+                    const int mid = (p0 + last) / 2;
+                    if (count(lo, lo + 1, mid) >= need) last = mid;
+                    else p0 = mid + 1;
+                }
+            }
+            for (int u = 0; u < n; u += UNIT) {
+                const char *pu = p + (int64_t)u * T::ESIZE;
+                for (uint32_t m = unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(lo)); m; m &= m - 1) {
+                    const int e = place(__ffs(m) - 1);
+                    const uint32_t key = beam_key<DT>(T::load1(pu, e));
+                    if (key > lo || u + e <= last) push(w, key, e0 + u + e);
+                }
+            }
+        }
+        __syncthreads();
+        m = s_m;
     }
+    for (int e = tid; e < m; e += BC_THREADS) {
+        const uint64_t t = cand[e].y;
+        const BeamRow &r = s_row[tie_beam(t)];
+        cand[e].x = beam_rank(r, beam_score(r, beam_x(a, r.ref, tie_key(t))), scaled);
+    }
+    if (tid < N) first[tid] = make_ulonglong2(0, 0);
     __syncthreads();
-    beam_sort(c_rank, c_tie, next_pow2(max(m, 2)));
+    beam_first(cand, m, a.pc, N, first, [](uint64_t) {});
     if (tid < N) {
         const int64_t o = (int64_t)blockIdx.x * N + tid;
-        float score = -__uint_as_float(0x7f800000u);
+        float score = NEG_INF;
         int parent = -1, token = -1, len = 0, done = 0;
         if (tid < m) {
-            const uint64_t t = c_tie[tid];
+            const uint64_t t = first[tid].y;
             const int w = tie_beam(t);
             const BeamRow &r = s_row[w];
-            score = (float)(a.alpha == 0.0 ? c_rank[tid] : beam_score(a, r, tie_key(t)));
+            score = scaled ? beam_score(r, beam_x(a, r.ref, tie_key(t))).h : key2f((uint32_t)(first[tid].x >> 32));
             parent = row0 + w;
             if (r.kind == BEAM_DONE) {
                 token = a.pad_token;
@@ -616,7 +881,7 @@ __global__ void __launch_bounds__(BC_THREADS) beam_combine_kernel(const BeamArgs
 }
 
 template <int DT, bool VEC, bool CAP>
-static cudaError_t launch_beam_t(const BeamArgs &a, int sms, cudaStream_t s)
+static cudaError_t launch_beam_t(BeamArgs &a, int sms, cudaStream_t s)
 {
     static int bps[MAX_DEVICES] = {};
     static bool ready[MAX_DEVICES] = {};
@@ -631,15 +896,19 @@ static cudaError_t launch_beam_t(const BeamArgs &a, int sms, cudaStream_t s)
         if (e != cudaSuccess) return e;
         ready[dev] = true;
     }
-    const int64_t items = (int64_t)a.rows * a.ipr, per = BS_THREADS / 32;
-    const int64_t blocks = (items + per - 1) / per, most = (int64_t)bps[dev] * sms;
+    const int64_t per = BS_THREADS / 32, most = (int64_t)bps[dev] * sms;
+    // items of two units (one load), longer ones where a row has over BEAM_MAX_ITEMS of them
+    const int unit = BeamGeo<DT>::UNIT, units = (a.vocab + unit - 1) / unit;
+    a.upi = 2 * ((units + 2 * BEAM_MAX_ITEMS - 1) / (2 * BEAM_MAX_ITEMS));
+    a.ipr = (units + a.upi - 1) / a.upi;
+    const int64_t items = (int64_t)a.rows * a.ipr, blocks = (items + per - 1) / per;
     beam_stream_kernel<DT, VEC, CAP><<<(unsigned)(blocks < most ? blocks : most), BS_THREADS, 0, s>>>(a);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows / a.beams));
     cfg.blockDim = dim3(BC_THREADS);
-    cfg.dynamicSmemBytes = (size_t)(a.pe + a.pc) * 16;
+    cfg.dynamicSmemBytes = (size_t)(a.pe + a.pc + a.n_out) * 16;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -649,15 +918,43 @@ static cudaError_t launch_beam_t(const BeamArgs &a, int sms, cudaStream_t s)
     return cudaLaunchKernelEx(&cfg, beam_combine_kernel<DT, VEC>, a);
 }
 
+// tanh(q) / q = 1 + q^2 P(q^2) on |q| <= 1/2, P of degree 3 fitted for the least largest
+// relative error (1.5e-8)
+static const double BEAM_TH[4] = {-0.3333314389543194, 0.13325878934833307, -0.05304549251234199, 0.017241487414783898};
+
 template <int DT>
-static cudaError_t launch_beam_dt(const BeamArgs &a, bool vec, int sms, cudaStream_t s)
+static cudaError_t launch_beam_dt(BeamArgs &a, bool vec, int sms, cudaStream_t s)
 {
     if (a.softcap > 0.0f) return vec ? launch_beam_t<DT, true, true>(a, sms, s) : launch_beam_t<DT, false, true>(a, sms, s);
     return vec ? launch_beam_t<DT, true, false>(a, sms, s) : launch_beam_t<DT, false, false>(a, sms, s);
 }
 
-cudaError_t launch_beam_select(const BeamArgs &a, int dtype, bool vec, int sms, cudaStream_t s)
+cudaError_t launch_beam_select(BeamArgs &a, int dtype, bool vec, int sms, cudaStream_t s)
 {
+    a.k = (float)a.k64;
+    a.ref32 = a.softcap > 0.0f ? 1.0f : a.k;
+    const double invcap = a.softcap > 0.0f ? 1.0 / (double)a.softcap : 0.0, invt = a.k64 * 0.69314718055994530942;
+    auto pair = [](double v, float (&o)[2]) {
+        o[0] = (float)v;
+        o[1] = (float)(v - (double)o[0]);
+    };
+    pair(invcap, a.invcap2);
+    pair(a.softcap > 0.0f ? a.softcap * invt : invt, a.scale2);
+    pair(a.alpha, a.alpha2);
+    a.invcap = (float)invcap;
+    // the folded coefficients stay normal numbers for caps of this range only
+    const bool fold = a.softcap >= 1e-2f && a.softcap <= 1e3f;
+    a.lim1 = fold ? 0.5f * a.softcap : -1.0f;
+    a.lim2 = fold ? a.softcap : -1.0f;
+    a.skip_min = fold && (double)a.softcap * invt >= 28.0;
+    static const double th[BEAM_H2 - 1] = {G4_TH0, G4_TH1, G4_TH2, G4_TH3, G4_TH4, G4_TH5, G4_TH6};
+    a.h1[0] = a.h2[0] = a.k;
+    double c = a.k64;
+    for (int i = 1; i < BEAM_H2; i++) {
+        c *= invcap * invcap;
+        a.h2[i] = (float)(c * th[i - 1]);
+        if (i < BEAM_H1) a.h1[i] = (float)(c * BEAM_TH[i - 1]);
+    }
     return dtype == G4S_F32 ? launch_beam_dt<G4S_F32>(a, vec, sms, s) : launch_beam_dt<G4S_BF16>(a, vec, sms, s);
 }
 

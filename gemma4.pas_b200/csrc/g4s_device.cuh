@@ -160,6 +160,16 @@ __device__ __forceinline__ uint4 ld_stream_v4(const void *p)
     return r;
 }
 
+// asynchronous copies of 16 bytes into shared memory
+__device__ __forceinline__ void cp_async16(void *smem, const void *gmem)
+{
+    const uint32_t sa = (uint32_t)__cvta_generic_to_shared(smem);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sa), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 template <int DT>
 struct DtypeTraits;
 template <>

@@ -307,15 +307,6 @@ __device__ __forceinline__ void stream_item(const SampleArgs &a, int64_t it, int
     if ((threadIdx.x & 31) == 0) a.istat[it] = make_float4(m, cc, S, redo ? 1.0f : 0.0f);
 }
 
-__device__ __forceinline__ void cp_async16(void *smem, const void *gmem)
-{
-    const uint32_t sa = (uint32_t)__cvta_generic_to_shared(smem);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sa), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Persistent streaming pass.  Warp w handles items w, w + W, w + 2W, ... (W =
 // warps in the grid).  With aligned rows each lane copies its own 16-byte
 // vectors of the items two ahead into a per-warp three-stage shared-memory ring

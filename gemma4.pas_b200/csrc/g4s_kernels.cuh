@@ -216,17 +216,17 @@ int full_etab_blocks_per_sm();
 // ---------------------------------------------------------------------------
 // beam search (g4s_beam.cu, g4s_pages.cu)
 // ---------------------------------------------------------------------------
-constexpr int BEAM_MAX_ITEMS = 512;  // items a row in the selection's statistics
-constexpr int BEAM_COMBINE_SMEM_MAX = (2048 + 4096) * 16;  // 32 beams, 64 continuations
+constexpr int BEAM_MAX_ITEMS = 128;  // items a row in the selection's statistics
+constexpr int BEAM_COMBINE_SMEM_MAX = (2048 + 4096 + 64) * 16;  // 32 beams, 64 continuations
+constexpr int BEAM_H1 = 5, BEAM_H2 = 8;  // coefficients of the folded softcap polynomials
 
 struct BeamArgs {
     const void *logits;
     int64_t row_stride;   // elements
     int rows, beams, vocab, n_out;
-    int upi, ipr;         // 2 KiB units an item, items a row
     int pe, pc;           // combine: sort sizes (powers of two) of the items and of the tokens
-    float softcap, invcap, k;  // k = log2(e) / temperature
-    double k64, temperature, alpha;
+    float softcap;        // 0: none
+    double k64, alpha;    // log2(e) / temperature
     int pad_token, n_eos, eos[G4S_BEAM_MAX_EOS];
     const float *scores;
     const int32_t *lens;
@@ -235,11 +235,16 @@ struct BeamArgs {
     int32_t *out_lens;
     uint8_t *out_done;
     int32_t *out_parents, *out_tokens;
-    float4 *istat;        // [rows][ipr] (m, c, S, -)
+    float4 *istat;        // [rows][ipr] (m, ref, S, -)
+    // set by launch_beam_select
+    int upi, ipr;         // 2 KiB units an item, items a row
+    float k, invcap, lim1, lim2;         // lim1, lim2: largest |logit| of the two polynomials
+    float ref32;                         // powers of two a unit of ref
+    int skip_min;                        // whether the first polynomial may take any logit below cap / 2
+    float invcap2[2], scale2[2], alpha2[2];  // 1 / cap, cap / T (or 1 / T) and alpha as pairs
+    float h1[BEAM_H1], h2[BEAM_H2];      // s(l) k = l H(l^2)
 };
-// Logits of a 2 KiB unit.
-int beam_unit_logits(int dtype);
-cudaError_t launch_beam_select(const BeamArgs &a, int dtype, bool vec, int sms, cudaStream_t s);
+cudaError_t launch_beam_select(BeamArgs &a, int dtype, bool vec, int sms, cudaStream_t s);
 
 constexpr int REORDER_THREADS = 256;
 struct ReorderTensor {

@@ -439,10 +439,11 @@ typedef struct g4s_beam_state {
  *   score = scores[beam] + x_i - log sum_j exp(x_j),
  * where a logit that is NaN or at or below -1e30 is masked (no candidate, no
  * mass; a row without any other has no candidate) and +inf counts as the
- * largest finite number.  An ended beam has one continuation: pad_token at its
+ * type's largest finite number.  An ended beam has one continuation: pad_token at its
  * own score and length.  Order: score / max(length after the token,
- * 1)^length_alpha, descending, computed in 64 bits; then the lower beam; within
- * a beam the larger logit, then the lower id.  Places that no continuation
+ * 1)^length_alpha, descending, the row's sum of exponentials being off by 1e-7
+ * or so; then the lower beam; within a beam the larger logit, then the lower
+ * id.  Places that no continuation
  * fills get score -inf, parent and token -1, length 0, done 0.
  *   logits        rows x row_stride elements, rows = groups * params->beams
  *   out_parents   [groups * n_out] the row continued (0..rows-1)

@@ -8,9 +8,9 @@ NEG = -np.inf
 EOS = (1, 106, 50)
 
 
-def select(logits, scores, lens, done, W, N, cap, T, alpha, pad=0, eos=EOS):
+def select(logits, scores, lens, done, W, N, cap, T, alpha, pad=0, eos=EOS, fmax=float(np.finfo(np.float32).max)):
     """g4s_beam_select of [rows, V] float64 logits: a list per group of (rank, score, row, token, len, done),
-    every candidate in order (not only the first N)."""
+    every candidate in order (not only the first N).  fmax: what +inf counts as."""
     rows, V = logits.shape
     out = []
     for g in range(rows // W):
@@ -31,7 +31,7 @@ def select(logits, scores, lens, done, W, N, cap, T, alpha, pad=0, eos=EOS):
             ok = np.nonzero(x > -1e30)[0]
             if ok.size == 0:
                 continue
-            v = np.minimum(x[ok], np.finfo(np.float32).max) + 0.0
+            v = np.minimum(x[ok], fmax) + 0.0
             s = cap * np.tanh(v / cap) if cap > 0 else v
             m = s.max()
             with np.errstate(over="ignore"):
