@@ -160,6 +160,17 @@ __device__ __forceinline__ uint4 ld_stream_v4(const void *p)
     return r;
 }
 
+// Reads a word of every 64 bytes of a kernel's parameters, so that the constant cache holds
+// them: each line's first use costs a few hundred cycles otherwise, one after another (a
+// kernel launched ahead of the one it depends on does it while it waits).
+template <class A>
+__device__ __forceinline__ void touch_params(const A &a)
+{
+    static_assert(sizeof(A) % 4 == 0, "words");
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(A) / 4; i += 16) asm volatile("" ::"r"(reinterpret_cast<const int *>(&a)[i]));
+}
+
 // asynchronous copies of 16 bytes into shared memory
 __device__ __forceinline__ void cp_async16(void *smem, const void *gmem)
 {

@@ -24,29 +24,29 @@ constexpr int PG_SLICES = PG_CLUSTER * PG_WARPS;  // a warp's slice of the page 
 constexpr int PC_THREADS = 256;     // CTA of the copies
 constexpr int PC_VECS = 4;          // vectors a thread and step
 
-// Exclusive scan over the CTA's PG_THREADS values; *total gets the sum.  sh: PG_WARPS + 1 ints.
-__device__ __forceinline__ int pg_scan(int v, int *total, int *sh)
+// Exclusive scan over the CTA's PG_THREADS values; *total gets the sum.  sh: PG_WARPS + 1.
+__device__ __forceinline__ unsigned long long pg_scan(unsigned long long v, unsigned long long *total, unsigned long long *sh)
 {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int inc = warp_incl_scan(v);
+    const unsigned long long inc = warp_incl_scan(v);
     if (lane == 31) sh[w] = inc;
     __syncthreads();
     if (w == 0) {
-        const int s = sh[lane];
-        const int si = warp_incl_scan(s);
+        const unsigned long long s = sh[lane], si = warp_incl_scan(s);
         sh[lane] = si - s;
         if (lane == 31) sh[PG_WARPS] = si;
     }
     __syncthreads();
-    const int r = sh[w] + inc - v;
+    const unsigned long long r = sh[w] + inc - v;
     *total = sh[PG_WARPS];
     __syncthreads();
     return r;
 }
 
-__device__ __forceinline__ int64_t pages_of(int64_t tokens, int page_tokens)
+// Pages of that many positions (each below 2^30, so sums of three fit in 32 bits).
+__device__ __forceinline__ int pages_of(int tokens, int page_tokens)
 {
-    return (tokens + page_tokens - 1) / page_tokens;
+    return (int)(((uint32_t)tokens + (uint32_t)page_tokens - 1) / (uint32_t)page_tokens);
 }
 
 // A sequence's length, or -1 where the table cannot hold it.
@@ -56,85 +56,114 @@ __device__ __forceinline__ int seq_len(const PagesArgs &a, int i)
     return n >= 0 && (int64_t)n <= (int64_t)a.width * a.page_tokens ? n : -1;
 }
 
-// Fork.  Dynamic shared memory, n = max(n_in, n_out): children of each old sequence, and
-// of each new one its length, last page if it has to be its own, its place in the
-// allocation and in the copies.
-__global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const PagesArgs a)
+// Fork.  Every CTA of the cluster works out the same sequences and needs in its own shared
+// memory; the old sequences' table rows and the pages' counts are split over the warps.
+constexpr int PG_ONE_PAGES = 8192, PG_ONE_ENTRIES = 8192;  // up to these one CTA decides
+constexpr int PG_HEADS = 1024;  // lists of the sequences that write to a page, by its id
+constexpr int PG_MASKS = 4;     // 32-page masks of its slice that a warp keeps
+constexpr int PG_ROW = 8;       // table entries a lane has under way
+
+__global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_constant__ PagesArgs a)
 {
     cg::cluster_group cluster = cg::this_cluster();
     extern __shared__ int s_dyn[];
-    __shared__ int s_free[PG_WARPS], s_sh[PG_WARPS + 1], s_pref[PG_SLICES], s_bad, s_over, s_allbad;
-    const int rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int gw = rank * PG_WARPS + warp, gt = rank * PG_THREADS + tid;
+    __shared__ int s_free[PG_WARPS], s_bad, s_over, s_writers[PG_HEADS];
+    __shared__ unsigned long long s_sh[PG_WARPS + 1];
+    const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int slices = nc * PG_WARPS, gw = rank * PG_WARPS + warp, gt = rank * PG_THREADS + tid;
     const int P = a.page_tokens, nmax = max(a.n_in, a.n_out);
-    int *s_kids = s_dyn, *s_len = s_kids + a.n_in, *s_last = s_len + nmax, *s_off = s_last + nmax, *s_cp = s_off + nmax;
+    int *s_len = s_dyn;         // [n_out] length, -1: an empty sequence
+    int *s_last = s_len + nmax; // [n_out] the partly filled last page it will write to, or -1
+    int *s_next = s_last + nmax;  // [n_out] next of its parent's children, then of its page's writers
+    int *s_off = s_next + nmax; // [n_in] first child of an old sequence; then [n_out] its place in the allocation
+    int *s_copy = s_off + nmax; // [n_out] its place among the copies, or -1
+    auto sync = [&] {
+        if (nc > 1) cluster.sync();
+        else __syncthreads();
+    };
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (tid == 0) s_bad = s_over = 0;
-    for (int i = tid; i < a.n_in; i += PG_THREADS) s_kids[i] = 0;
-    if (a.refs_out != a.refs_in)
-        for (int p = gt; p < a.n_pages; p += PG_CLUSTER * PG_THREADS) a.refs_out[p] = a.refs_in[p];
+    for (int i = tid; i < a.n_in; i += PG_THREADS) s_off[i] = -1;
+    s_writers[tid] = -1;
+    static_assert(PG_HEADS == PG_THREADS, "one list head a thread");
+    touch_params(a);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     __syncthreads();
+    if (a.refs_out != a.refs_in)
+        for (int p = gt; p < a.n_pages; p += nc * PG_THREADS) a.refs_out[p] = a.refs_in[p];
     for (int j = tid; j < a.n_out; j += PG_THREADS) {
         const int p = a.src[j];
-        int len = 0;
+        int len = -1, last = -1;
         if (p >= 0) {
             len = p < a.n_in ? seq_len(a, p) : -1;
-            if (len >= 0) atomicAdd(&s_kids[p], 1);
+            if (len >= 0) s_next[j] = atomicExch(&s_off[p], j);
             else if (rank == 0) atomicAdd(&s_bad, 1);
+            if (a.n_new > 0 && len > 0 && len % P && !(a.frozen && a.frozen[j])) {
+                last = a.tables_in[(int64_t)p * a.width + len / P];
+                if (last < 0 || last >= a.n_pages) last = -1;
+            }
         }
-        s_len[j] = p >= 0 && len >= 0 ? len : -1;  // -1: an empty sequence
-    }
-    cluster.sync();  // the counts are copied
-
-    // each old sequence's pages lose its hold and gain its children's
-    for (int i = gw; i < a.n_in; i += PG_SLICES) {
-        const int d = s_kids[i] - 1, len = seq_len(a, i);
-        if (d == 0 || len <= 0) continue;
-        const int32_t *row = a.tables_in + (int64_t)i * a.width;
-        for (int c = lane; c < pages_of(len, P); c += 32) {
-            const int p = row[c];
-            if (p >= 0 && p < a.n_pages) atomicAdd(&a.refs_out[p], d);
-        }
-    }
-    for (int j = gw; j < a.n_out; j += PG_SLICES) {
-        if (s_len[j] <= 0) continue;
-        const int32_t *row = a.tables_in + (int64_t)a.src[j] * a.width;
-        int32_t *to = a.tables_out + (int64_t)j * a.width;
-        int bad = 0;
-        for (int c = lane; c < pages_of(s_len[j], P); c += 32) {
-            const int p = row[c];
-            to[c] = p;
-            bad += p < 0 || p >= a.n_pages;
-        }
-        bad = __reduce_add_sync(FULLMASK, bad);
-        if (lane == 0 && bad) atomicAdd(&s_bad, bad);
-    }
-    cluster.sync();  // the counts are the fork's
-
-    // free pages of each warp's slice
-    const int per = (a.n_pages + PG_SLICES - 1) / PG_SLICES;
-    const int64_t lo = (int64_t)gw * per;
-    const int n_slice = (int)max((int64_t)0, min((int64_t)per, a.n_pages - lo));
-    {
-        int n = 0;
-        for (int i = lane; i < n_slice; i += 32) n += __ldcg(a.refs_out + lo + i) <= 0;
-        n = __reduce_add_sync(FULLMASK, n);
-        if (lane == 0) s_free[warp] = n;
-    }
-    // every CTA works out every sequence's needs (a page that only one holds stays its
-    // own; of w writers of a page with r holds, the first min(w, r - 1) copy it)
-    for (int j = tid; j < a.n_out; j += PG_THREADS) {
-        const int len = s_len[j];
-        int last = -1;
-        if (a.n_new > 0 && len > 0 && len % P && !(a.frozen && a.frozen[j])) {
-            last = a.tables_in[(int64_t)a.src[j] * a.width + len / P];
-            if (last < 0 || last >= a.n_pages) last = -1;
-        }
+        s_len[j] = len;
         s_last[j] = last;
     }
+    sync();  // the counts are copied, the children listed
+
+    // each old sequence's row goes to its children; its pages lose its hold and gain theirs
+    for (int i = gw; i < a.n_in; i += slices) {
+        const int n = pages_of(max(seq_len(a, i), 0), P), first = s_off[i];
+        int kids = 0;
+        for (int j = first; j >= 0; j = s_next[j]) kids++;
+        const int32_t *row = a.tables_in + (int64_t)i * a.width;
+        int bad = 0;
+        for (int c0 = lane; c0 < n; c0 += PG_ROW * 32) {
+            int v[PG_ROW];
+#pragma unroll
+            for (int k = 0; k < PG_ROW; k++) v[k] = c0 + k * 32 < n ? row[c0 + k * 32] : 0;
+#pragma unroll
+            for (int k = 0; k < PG_ROW; k++) {
+                const bool in = c0 + k * 32 < n, page = v[k] >= 0 && v[k] < a.n_pages;
+                if (in && page && kids != 1) atomicAdd(&a.refs_out[v[k]], kids - 1);
+                bad += in && !page;
+            }
+            for (int j = first; j >= 0; j = s_next[j]) {
+                int32_t *to = a.tables_out + (int64_t)j * a.width;
+#pragma unroll
+                for (int k = 0; k < PG_ROW; k++)
+                    if (c0 + k * 32 < n) to[c0 + k * 32] = v[k];
+            }
+        }
+        bad = __reduce_add_sync(FULLMASK, bad);
+        if (lane == 0 && bad) atomicAdd(&s_bad, bad * kids);
+    }
+    sync();  // the counts are the fork's
+
+    // free pages of each warp's slice
+    const int per = (a.n_pages + slices - 1) / slices;
+    const int64_t lo = (int64_t)gw * per;
+    const int n_slice = (int)max((int64_t)0, min((int64_t)per, a.n_pages - lo));
+    unsigned free_mask[PG_MASKS];  // of the slice's first pages
+    {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < PG_MASKS; k++) {
+            const int i = k * 32 + lane;
+            free_mask[k] = __ballot_sync(FULLMASK, i < n_slice && __ldcg(a.refs_out + lo + i) <= 0);
+            n += __popc(free_mask[k]);
+        }
+        for (int i0 = PG_MASKS * 32; i0 < n_slice; i0 += 32) {
+            const int i = i0 + lane;
+            n += __popc(__ballot_sync(FULLMASK, i < n_slice && __ldcg(a.refs_out + lo + i) <= 0));
+        }
+        if (lane == 0) s_free[warp] = n;
+    }
+    for (int j = tid; j < a.n_out; j += PG_THREADS)
+        if (s_last[j] >= 0) s_next[j] = atomicExch(&s_writers[s_last[j] % PG_HEADS], j);
     __syncthreads();
-    int base = 0, cbase = 0;
+    // every sequence's needs (a page that only one holds stays its own; of w writers of a
+    // page with r holds, the first min(w, r - 1) copy it)
+    unsigned long long base = 0;  // copies << 40 | pages
     for (int j0 = 0; j0 < a.n_out; j0 += PG_THREADS) {
         const int j = j0 + tid;
         int need = 0, copy = 0;
@@ -144,58 +173,64 @@ __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS,
                 const int holds = __ldcg(a.refs_out + last);
                 if (holds > 1) {
                     int before = 0;
-                    for (int i = 0; i < j; i++) before += s_last[i] == last;
+                    for (int i = s_writers[last % PG_HEADS]; i >= 0; i = s_next[i]) before += s_last[i] == last && i < j;
                     copy = before < holds - 1;
                 }
             }
-            const int64_t now = pages_of(len, P), then = pages_of((int64_t)len + a.n_new, P);
+            const int now = pages_of(len, P), then = pages_of(len + a.n_new, P);
             if (then > a.width) {
                 if (rank == 0) atomicAdd(&s_over, 1);
             } else {
-                need = copy + (int)(then - now);
+                need = copy + (then - now);
             }
         }
-        int total, ctotal;
-        const int off = pg_scan(need, &total, s_sh), coff = pg_scan(copy, &ctotal, s_sh);
+        unsigned long long total;
+        const unsigned long long off = base + pg_scan((unsigned long long)copy << 40 | (uint32_t)need, &total, s_sh);
         if (j < a.n_out) {
-            s_off[j] = base + off;
-            s_cp[j] = copy ? cbase + coff : -1;
+            s_off[j] = (int)min(off & ((1ull << 40) - 1), 0x7fffffffull);
+            s_copy[j] = copy ? (int)(off >> 40) : -1;
         }
         base += total;
-        cbase += ctotal;
     }
-    cluster.sync();  // the slices' free pages, the bad entries
+    const int64_t taken = (int64_t)(base & ((1ull << 40) - 1));
+    sync();  // the slices' free pages, the bad entries
 
-    if (tid < PG_SLICES) s_pref[tid] = *cluster.map_shared_rank(&s_free[tid % PG_WARPS], tid / PG_WARPS);
-    if (tid == PG_SLICES) {
-        int bad = 0;
-        for (int r = 0; r < PG_CLUSTER; r++) bad += *cluster.map_shared_rank(&s_bad, r);
-        s_allbad = bad;
+    // free pages in all, and before the warp's slice
+    int free_pages = 0, k0 = 0, bad = 0;
+    for (int i = lane; i < slices; i += 32) {
+        const int n = nc > 1 ? *cluster.map_shared_rank(&s_free[i % PG_WARPS], i / PG_WARPS) : s_free[i];
+        free_pages += n;
+        k0 += i < gw ? n : 0;
     }
-    if (tid == PG_SLICES + 1 && rank) s_over = *cluster.map_shared_rank(&s_over, 0);
-    __syncthreads();
-    int free_pages;
-    const int pref = pg_scan(tid < PG_SLICES ? s_pref[tid] : 0, &free_pages, s_sh);
-    if (tid < PG_SLICES) s_pref[tid] = pref;
-    __syncthreads();
-    const bool ok = base <= free_pages && s_over == 0 && s_allbad == 0;
-    if (ok && s_pref[gw] < base) {
+    if (lane < nc) bad = nc > 1 ? *cluster.map_shared_rank(&s_bad, lane) : s_bad;
+    const int over = nc > 1 ? *cluster.map_shared_rank(&s_over, 0) : s_over;
+    free_pages = __reduce_add_sync(FULLMASK, free_pages);
+    k0 = __reduce_add_sync(FULLMASK, k0);
+    bad = __reduce_add_sync(FULLMASK, bad);
+    if (nc > 1) cluster.barrier_arrive();  // (this CTA has read the others' shared memory)
+    const bool ok = taken <= free_pages && over == 0 && bad == 0;
+    if (ok && k0 < taken) {
         // the k-th free page belongs to the last sequence whose place is at or before k
-        int k0 = s_pref[gw];
-        for (int i0 = 0; i0 < n_slice && k0 < base; i0 += 32) {
+        for (int i0 = 0; i0 < n_slice && k0 < taken; i0 += 32) {
             const int p = (int)lo + i0 + lane;
-            const bool is = i0 + lane < n_slice && __ldcg(a.refs_out + p) <= 0;
-            const unsigned b = __ballot_sync(FULLMASK, is);
+            unsigned b = 0;
+            if (i0 < PG_MASKS * 32) {
+#pragma unroll
+                for (int k = 0; k < PG_MASKS; k++) b = i0 == k * 32 ? free_mask[k] : b;
+            } else {
+                b = __ballot_sync(FULLMASK, i0 + lane < n_slice && __ldcg(a.refs_out + p) <= 0);
+            }
+            const bool is = b >> lane & 1;
             const int k = k0 + __popc(b & ((1u << lane) - 1));
             k0 += __popc(b);
-            if (!is || k >= base) continue;
+            if (!is || k >= taken) continue;
             int j = 0, hi = a.n_out - 1;
             while (j < hi) {
                 const int mid = (j + hi + 1) / 2;
                 if (s_off[mid] <= k) j = mid;
                 else hi = mid - 1;
             }
-            const int len = s_len[j], t = k - s_off[j], slot = s_cp[j];
+            const int len = s_len[j], t = k - s_off[j], slot = s_copy[j];
             a.refs_out[p] = 1;
             if (slot >= 0 && t == 0) {
                 a.tables_out[(int64_t)j * a.width + len / P] = p;
@@ -213,14 +248,14 @@ __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS,
             a.lens_out[j] = len + (grows ? a.n_new : 0);
         }
         if (tid == 0) {
-            a.result[0] = ok ? base : 0;
-            a.result[1] = max(base - free_pages, 0);
-            a.result[2] = s_over;
-            a.result[3] = s_allbad;
-            *a.n_copies = ok ? cbase : 0;
+            a.result[0] = ok ? (int)taken : 0;
+            a.result[1] = (int)min(max(taken - free_pages, (int64_t)0), (int64_t)0x7fffffff);
+            a.result[2] = over;
+            a.result[3] = bad;
+            *a.n_copies = ok ? (int)(base >> 40) : 0;
         }
     }
-    cluster.sync();  // no CTA leaves while another reads its shared memory
+    if (nc > 1) cluster.barrier_wait();  // no CTA leaves while another may read its shared memory
 }
 
 // Compaction: used pages at or above the number of used pages go to the free pages below
@@ -228,7 +263,8 @@ __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS,
 __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(const PagesArgs a)
 {
     cg::cluster_group cluster = cg::this_cluster();
-    __shared__ int s_used[PG_WARPS], s_sh[PG_WARPS + 1], s_mv[PG_SLICES], s_ho[PG_SLICES], s_cut[2];
+    __shared__ int s_used[PG_WARPS], s_mv[PG_SLICES], s_ho[PG_SLICES], s_cut[2];
+    __shared__ unsigned long long s_sh[PG_WARPS + 1];
     const int rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gw = rank * PG_WARPS + warp, gt = rank * PG_THREADS + tid;
     const int per = (a.n_pages + PG_SLICES - 1) / PG_SLICES;
@@ -242,9 +278,10 @@ __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS,
     if (lane == 0) s_used[warp] = n;
     if (tid < 2) s_cut[tid] = 0;
     cluster.sync();
-    int used;
+    unsigned long long sum;
     const int mine = tid < PG_SLICES ? *cluster.map_shared_rank(&s_used[tid % PG_WARPS], tid / PG_WARPS) : 0;
-    pg_scan(mine, &used, s_sh);
+    pg_scan(mine, &sum, s_sh);
+    const int used = (int)sum;
     // pages to move and holes of every slice; the one that holds the border is counted again
     const int cut = used / per;  // its slice (every page used: none)
     for (int64_t p = (int64_t)cut * per + tid; p < min((int64_t)(cut + 1) * per, (int64_t)a.n_pages); p += PG_THREADS) {
@@ -264,11 +301,11 @@ __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS,
             holes = (int)max((int64_t)0, min((int64_t)per, (int64_t)a.n_pages - (int64_t)tid * per)) - mine;
         }
     }
-    int total, htotal;
-    const int mo = pg_scan(moves, &total, s_sh), ho = pg_scan(holes, &htotal, s_sh);
+    const unsigned long long before = pg_scan((unsigned long long)holes << 32 | (unsigned)moves, &sum, s_sh);
+    const int total = (int)(uint32_t)sum;
     if (tid < PG_SLICES) {
-        s_mv[tid] = mo;
-        s_ho[tid] = ho;
+        s_mv[tid] = (int)(uint32_t)before;
+        s_ho[tid] = (int)(before >> 32);
     }
     __syncthreads();
     int m0 = s_mv[gw], h0 = s_ho[gw];
@@ -328,8 +365,9 @@ __device__ __forceinline__ void copy_chunk(const PoolArg &q, int from, int to, i
 // The listed pages' contents, pool by pool: a fork copies the filled positions of its
 // copies, a compaction whole pages (and renames the tables' entries).
 template <bool FORK>
-__global__ void __launch_bounds__(PC_THREADS) pages_copy_kernel(const PagesArgs a, const PoolArgs pools)
+__global__ void __launch_bounds__(PC_THREADS) pages_copy_kernel(const __grid_constant__ PagesArgs a, const __grid_constant__ PoolArgs pools)
 {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if constexpr (!FORK) {
         for (int i = blockIdx.x; i < a.n_in; i += gridDim.x) {
@@ -373,7 +411,7 @@ __global__ void __launch_bounds__(PC_THREADS) pages_copy_kernel(const PagesArgs 
 
 int pages_chunk_vecs() { return PC_THREADS * PC_VECS; }
 
-int pages_fork_smem(int n_in, int n_out) { return (n_in + 4 * (n_in > n_out ? n_in : n_out)) * (int)sizeof(int); }
+int pages_fork_smem(int n_in, int n_out) { return 5 * (n_in > n_out ? n_in : n_out) * (int)sizeof(int); }
 
 template <bool FORK>
 static cudaError_t launch_copy(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s)
@@ -401,8 +439,22 @@ cudaError_t launch_pages_fork(const PagesArgs &a, const PoolArgs &pools, int sms
         const cudaError_t e = cudaFuncSetAttribute(pages_fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
     }
-    pages_fork_kernel<<<PG_CLUSTER, PG_THREADS, smem, s>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    // one CTA for few pages and table entries: its barriers are cheaper than the cluster's
+    const int nc = a.n_pages <= PG_ONE_PAGES && (int64_t)a.n_in * a.width <= PG_ONE_ENTRIES ? 1 : PG_CLUSTER;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)nc);
+    cfg.blockDim = dim3(PG_THREADS);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)nc;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, pages_fork_kernel, a);
     if (e != cudaSuccess || a.n_new == 0) return e;
     return launch_copy<true>(a, pools, sms, s);
 }
