@@ -1655,6 +1655,7 @@ int32_t g4s_pages_compact(g4s_ctx *ctx, const g4s_page_cache *cache, int32_t n_s
     if (!in || !out || !page_map || !moves || !result || !in->refs || !out->refs ||
         (n_seqs && (!in->tables || !in->lens || !out->tables)))
         return fail(ctx, G4S_ERR_ARG, "%s: in, out, their arrays, page_map, moves and result must be non-NULL", who);
+    if ((uintptr_t)moves % 8) return fail(ctx, G4S_ERR_ARG, "%s: moves is not 8-byte aligned", who);
     const size_t w = (size_t)n_seqs * a.width * 4, np = (size_t)a.n_pages * 4;
     if ((n_seqs && !aliasing_ok(in->tables, out->tables, w, w, true)) || !aliasing_ok(in->refs, out->refs, np, np, true))
         return fail(ctx, G4S_ERR_ARG, "%s: out's tables or refs overlap in's (allowed: the same arrays)", who);

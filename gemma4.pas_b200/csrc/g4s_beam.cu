@@ -313,7 +313,10 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
     uint64_t h1[BEAM_H1], k2 = two(a.k);
 #pragma unroll
     for (int i = 0; i < BEAM_H1; i++) h1[i] = CAP ? two(a.h1[i]) : 0;
-    Load cur = find(w0 / a.ipr, w0 % a.ipr), nx = after(cur);
+    touch_params(a);
+    const int row0 = w0 / a.ipr, item0 = w0 % a.ipr;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Load cur = find(row0, item0), nx = after(cur);
     float m = NEG_INF, ref = 0.0f;
     uint64_t s0 = 0, s1 = 0;
     uint32_t at = ring;
@@ -641,6 +644,7 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int W = a.beams, N = a.n_out, row0 = (int)blockIdx.x * W;
 
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     for (int e = tid; e < a.pe + a.pc + N; e += BC_THREADS) s_mem[e] = make_ulonglong2(0, 0);
     if (tid < G4S_BEAM_MAX) {
         s_least[tid] = BEAM_KEY_MIN;
@@ -915,20 +919,9 @@ static cudaError_t launch_beam_t(BeamArgs &a, int sms, cudaStream_t s)
     a.upi = 2 * ((units + 2 * BEAM_MAX_ITEMS - 1) / (2 * BEAM_MAX_ITEMS));
     a.ipr = (units + a.upi - 1) / a.upi;
     const int64_t items = (int64_t)a.rows * a.ipr, blocks = (items + per - 1) / per;
-    beam_stream_kernel<DT, VEC, CAP><<<(unsigned)(blocks < most ? blocks : most), BS_THREADS, 0, s>>>(a);
-    e = cudaGetLastError();
+    e = launch_dependent(beam_stream_kernel<DT, VEC, CAP>, blocks < most ? blocks : most, BS_THREADS, 0, s, a);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.rows / a.beams));
-    cfg.blockDim = dim3(BC_THREADS);
-    cfg.dynamicSmemBytes = (size_t)(a.pe + a.pc + a.n_out) * 16;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, beam_combine_kernel<DT, VEC>, a);
+    return launch_dependent(beam_combine_kernel<DT, VEC>, a.rows / a.beams, BC_THREADS, (size_t)(a.pe + a.pc + a.n_out) * 16, s, a);
 }
 
 // tanh(q) / q = 1 + q^2 P(q^2) on |q| <= 1/2, P of degree 3 fitted for the least largest
@@ -996,15 +989,17 @@ __device__ __forceinline__ void reorder_column(const ReorderTensor &t, int row0,
 }
 
 template <int WMAX>
-__global__ void __launch_bounds__(REORDER_THREADS) beam_reorder_kernel(const ReorderArgs a)
+__global__ void __launch_bounds__(REORDER_THREADS) beam_reorder_kernel(const __grid_constant__ ReorderArgs a)
 {
     __shared__ uint32_t s_child[WMAX];  // rows of the group that take row p's state
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int W = a.beams;
     int i = 0;
     while (i + 1 < a.n && (int64_t)blockIdx.x >= a.first[i + 1]) i++;
     const ReorderTensor &t = a.t[i];
     const int64_t b = (int64_t)blockIdx.x - a.first[i];
     const int row0 = (int)(b / t.blocks) * W;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (threadIdx.x < WMAX) {
         uint32_t m = 0;
         for (int j = 0; j < W; j++) {
@@ -1023,12 +1018,10 @@ __global__ void __launch_bounds__(REORDER_THREADS) beam_reorder_kernel(const Reo
 
 cudaError_t launch_beam_reorder(const ReorderArgs &a, int64_t blocks, cudaStream_t s)
 {
-    const unsigned g = (unsigned)blocks;
-    if (a.beams <= 4) beam_reorder_kernel<4><<<g, REORDER_THREADS, 0, s>>>(a);
-    else if (a.beams <= 8) beam_reorder_kernel<8><<<g, REORDER_THREADS, 0, s>>>(a);
-    else if (a.beams <= 16) beam_reorder_kernel<16><<<g, REORDER_THREADS, 0, s>>>(a);
-    else beam_reorder_kernel<32><<<g, REORDER_THREADS, 0, s>>>(a);
-    return cudaGetLastError();
+    if (a.beams <= 4) return launch_dependent(beam_reorder_kernel<4>, blocks, REORDER_THREADS, 0, s, a);
+    if (a.beams <= 8) return launch_dependent(beam_reorder_kernel<8>, blocks, REORDER_THREADS, 0, s, a);
+    if (a.beams <= 16) return launch_dependent(beam_reorder_kernel<16>, blocks, REORDER_THREADS, 0, s, a);
+    return launch_dependent(beam_reorder_kernel<32>, blocks, REORDER_THREADS, 0, s, a);
 }
 
 }  // namespace g4s

@@ -216,6 +216,26 @@ int full_etab_blocks_per_sm();
 // ---------------------------------------------------------------------------
 // beam search (g4s_beam.cu, g4s_pages.cu)
 // ---------------------------------------------------------------------------
+// Launches a kernel that may start before what precedes it on the stream has ended (a
+// programmatic dependent): it waits for that itself, with griddepcontrol.wait, before it
+// touches memory.
+template <class... P, class... A>
+inline cudaError_t launch_dependent(void (*kernel)(P...), int64_t blocks, int threads, size_t smem, cudaStream_t s,
+                                    const A &...args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 constexpr int BEAM_MAX_ITEMS = 128;  // items a row in the selection's statistics
 constexpr int BEAM_COMBINE_SMEM_MAX = (2048 + 4096 + 64) * 16;  // 32 beams, 64 continuations
 constexpr int BEAM_H1 = 5, BEAM_H2 = 8;  // coefficients of the folded softcap polynomials

@@ -17,30 +17,25 @@ namespace cg = cooperative_groups;
 
 namespace g4s {
 
-constexpr int PG_CLUSTER = 8;       // CTAs of the cluster that decides
+constexpr int PG_CLUSTER = 16;      // CTAs of the cluster that decides (16: a non-portable size)
 constexpr int PG_THREADS = 1024;
 constexpr int PG_WARPS = PG_THREADS / 32;
 constexpr int PG_SLICES = PG_CLUSTER * PG_WARPS;  // a warp's slice of the page counts
 constexpr int PC_THREADS = 256;     // CTA of the copies
 constexpr int PC_VECS = 4;          // vectors a thread and step
+constexpr int PC_CTAS = 6;          // CTAs on an SM
 
-// Exclusive scan over the CTA's PG_THREADS values; *total gets the sum.  sh: PG_WARPS + 1.
+// Exclusive scan over the CTA's PG_THREADS values; *total gets the sum.  sh: PG_WARPS, not
+// written again before the next barrier.
 __device__ __forceinline__ unsigned long long pg_scan(unsigned long long v, unsigned long long *total, unsigned long long *sh)
 {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const unsigned long long inc = warp_incl_scan(v);
     if (lane == 31) sh[w] = inc;
     __syncthreads();
-    if (w == 0) {
-        const unsigned long long s = sh[lane], si = warp_incl_scan(s);
-        sh[lane] = si - s;
-        if (lane == 31) sh[PG_WARPS] = si;
-    }
-    __syncthreads();
-    const unsigned long long r = sh[w] + inc - v;
-    *total = sh[PG_WARPS];
-    __syncthreads();
-    return r;
+    const unsigned long long s = sh[lane], si = warp_incl_scan(s);
+    *total = __shfl_sync(FULLMASK, si, 31);
+    return __shfl_sync(FULLMASK, si - s, w) + inc - v;
 }
 
 // Pages of that many positions (each below 2^30, so sums of three fit in 32 bits).
@@ -61,22 +56,24 @@ __device__ __forceinline__ int seq_len(const PagesArgs &a, int i)
 constexpr int PG_ONE_PAGES = 8192, PG_ONE_ENTRIES = 8192;  // up to these one CTA decides
 constexpr int PG_HEADS = 1024;  // lists of the sequences that write to a page, by its id
 constexpr int PG_MASKS = 4;     // 32-page masks of its slice that a warp keeps
-constexpr int PG_ROW = 8;       // table entries a lane has under way
+constexpr int PG_ROW = 4;       // table entries a lane has under way
 
 __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_constant__ PagesArgs a)
 {
     cg::cluster_group cluster = cg::this_cluster();
     extern __shared__ int s_dyn[];
     __shared__ int s_free[PG_WARPS], s_bad, s_over, s_writers[PG_HEADS];
-    __shared__ unsigned long long s_sh[PG_WARPS + 1];
+    __shared__ int4 s_cta[PG_CLUSTER];  // each CTA's free pages, bad entries, short tables
+    __shared__ unsigned long long s_sh[2][PG_WARPS];
     const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int slices = nc * PG_WARPS, gw = rank * PG_WARPS + warp, gt = rank * PG_THREADS + tid;
     const int P = a.page_tokens, nmax = max(a.n_in, a.n_out);
     int *s_len = s_dyn;         // [n_out] length, -1: an empty sequence
     int *s_last = s_len + nmax; // [n_out] the partly filled last page it will write to, or -1
-    int *s_next = s_last + nmax;  // [n_out] next of its parent's children, then of its page's writers
-    int *s_off = s_next + nmax; // [n_in] first child of an old sequence; then [n_out] its place in the allocation
+    int *s_next = s_last + nmax;  // [n_out] next of its parent's children
+    int *s_also = s_next + nmax;  // [n_out] next of that page's writers
+    int *s_off = s_also + nmax; // [n_in] first child of an old sequence; then [n_out] its place in the allocation
     int *s_copy = s_off + nmax; // [n_out] its place among the copies, or -1
     auto sync = [&] {
         if (nc > 1) cluster.sync();
@@ -103,6 +100,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
             if (a.n_new > 0 && len > 0 && len % P && !(a.frozen && a.frozen[j])) {
                 last = a.tables_in[(int64_t)p * a.width + len / P];
                 if (last < 0 || last >= a.n_pages) last = -1;
+                else s_also[j] = atomicExch(&s_writers[last % PG_HEADS], j);
             }
         }
         s_len[j] = len;
@@ -111,28 +109,26 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
     sync();  // the counts are copied, the children listed
 
     // each old sequence's row goes to its children; its pages lose its hold and gain theirs
-    for (int i = gw; i < a.n_in; i += slices) {
+    const int chunks = (a.width + PG_ROW * 32 - 1) / (PG_ROW * 32);
+    for (int task = gw; task < a.n_in * chunks; task += slices) {
+        const int i = task / chunks, c0 = task % chunks * (PG_ROW * 32) + lane;
         const int n = pages_of(max(seq_len(a, i), 0), P), first = s_off[i];
-        int kids = 0;
-        for (int j = first; j >= 0; j = s_next[j]) kids++;
-        const int32_t *row = a.tables_in + (int64_t)i * a.width;
-        int bad = 0;
-        for (int c0 = lane; c0 < n; c0 += PG_ROW * 32) {
-            int v[PG_ROW];
+        if (c0 - lane >= n) continue;
+        const int32_t *row = a.tables_in + (int64_t)i * a.width + c0;
+        int v[PG_ROW], bad = 0, kids = 0;
 #pragma unroll
-            for (int k = 0; k < PG_ROW; k++) v[k] = c0 + k * 32 < n ? row[c0 + k * 32] : 0;
+        for (int k = 0; k < PG_ROW; k++) v[k] = c0 + k * 32 < n ? row[k * 32] : 0;
+        for (int j = first; j >= 0; j = s_next[j], kids++) {
+            int32_t *to = a.tables_out + (int64_t)j * a.width + c0;
 #pragma unroll
-            for (int k = 0; k < PG_ROW; k++) {
-                const bool in = c0 + k * 32 < n, page = v[k] >= 0 && v[k] < a.n_pages;
-                if (in && page && kids != 1) atomicAdd(&a.refs_out[v[k]], kids - 1);
-                bad += in && !page;
-            }
-            for (int j = first; j >= 0; j = s_next[j]) {
-                int32_t *to = a.tables_out + (int64_t)j * a.width;
+            for (int k = 0; k < PG_ROW; k++)
+                if (c0 + k * 32 < n) to[k * 32] = v[k];
+        }
 #pragma unroll
-                for (int k = 0; k < PG_ROW; k++)
-                    if (c0 + k * 32 < n) to[c0 + k * 32] = v[k];
-            }
+        for (int k = 0; k < PG_ROW; k++) {
+            const bool in = c0 + k * 32 < n, page = v[k] >= 0 && v[k] < a.n_pages;
+            if (in && page && kids != 1) atomicAdd(&a.refs_out[v[k]], kids - 1);
+            bad += in && !page;
         }
         bad = __reduce_add_sync(FULLMASK, bad);
         if (lane == 0 && bad) atomicAdd(&s_bad, bad * kids);
@@ -143,6 +139,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
     const int per = (a.n_pages + slices - 1) / slices;
     const int64_t lo = (int64_t)gw * per;
     const int n_slice = (int)max((int64_t)0, min((int64_t)per, a.n_pages - lo));
+    const int holds0 = tid < a.n_out && s_last[tid] >= 0 ? __ldcg(a.refs_out + s_last[tid]) : 0;  // (under way early)
     unsigned free_mask[PG_MASKS];  // of the slice's first pages
     {
         int n = 0;
@@ -158,9 +155,6 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
         }
         if (lane == 0) s_free[warp] = n;
     }
-    for (int j = tid; j < a.n_out; j += PG_THREADS)
-        if (s_last[j] >= 0) s_next[j] = atomicExch(&s_writers[s_last[j] % PG_HEADS], j);
-    __syncthreads();
     // every sequence's needs (a page that only one holds stays its own; of w writers of a
     // page with r holds, the first min(w, r - 1) copy it)
     unsigned long long base = 0;  // copies << 40 | pages
@@ -170,10 +164,10 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
         if (j < a.n_out && s_len[j] >= 0 && a.n_new > 0 && !(a.frozen && a.frozen[j])) {
             const int len = s_len[j], last = s_last[j];
             if (last >= 0) {
-                const int holds = __ldcg(a.refs_out + last);
+                const int holds = j0 == 0 ? holds0 : __ldcg(a.refs_out + last);
                 if (holds > 1) {
                     int before = 0;
-                    for (int i = s_writers[last % PG_HEADS]; i >= 0; i = s_next[i]) before += s_last[i] == last && i < j;
+                    for (int i = s_writers[last % PG_HEADS]; i >= 0; i = s_also[i]) before += s_last[i] == last && i < j;
                     copy = before < holds - 1;
                 }
             }
@@ -185,7 +179,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
             }
         }
         unsigned long long total;
-        const unsigned long long off = base + pg_scan((unsigned long long)copy << 40 | (uint32_t)need, &total, s_sh);
+        const unsigned long long off = base + pg_scan((unsigned long long)copy << 40 | (uint32_t)need, &total, s_sh[j0 / PG_THREADS % 2]);
         if (j < a.n_out) {
             s_off[j] = (int)min(off & ((1ull << 40) - 1), 0x7fffffffull);
             s_copy[j] = copy ? (int)(off >> 40) : -1;
@@ -193,21 +187,20 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
         base += total;
     }
     const int64_t taken = (int64_t)(base & ((1ull << 40) - 1));
-    sync();  // the slices' free pages, the bad entries
-
-    // free pages in all, and before the warp's slice
-    int free_pages = 0, k0 = 0, bad = 0;
-    for (int i = lane; i < slices; i += 32) {
-        const int n = nc > 1 ? *cluster.map_shared_rank(&s_free[i % PG_WARPS], i / PG_WARPS) : s_free[i];
-        free_pages += n;
-        k0 += i < gw ? n : 0;
+    __syncthreads();
+    // each CTA's free pages, bad entries and short tables into every CTA's shared memory
+    if (warp == 0) {
+        const int n = __reduce_add_sync(FULLMASK, s_free[lane]);
+        if (lane < nc) {
+            int4 *to = nc > 1 ? cluster.map_shared_rank(s_cta, lane) : s_cta;
+            to[rank] = make_int4(n, s_bad, s_over, 0);
+        }
     }
-    if (lane < nc) bad = nc > 1 ? *cluster.map_shared_rank(&s_bad, lane) : s_bad;
-    const int over = nc > 1 ? *cluster.map_shared_rank(&s_over, 0) : s_over;
-    free_pages = __reduce_add_sync(FULLMASK, free_pages);
-    k0 = __reduce_add_sync(FULLMASK, k0);
-    bad = __reduce_add_sync(FULLMASK, bad);
-    if (nc > 1) cluster.barrier_arrive();  // (this CTA has read the others' shared memory)
+    sync();
+    const int4 cta = lane < nc ? s_cta[lane] : make_int4(0, 0, 0, 0);
+    const int free_pages = __reduce_add_sync(FULLMASK, cta.x), bad = __reduce_add_sync(FULLMASK, cta.y);
+    const int over = __reduce_add_sync(FULLMASK, cta.z);  // (counted by the first CTA alone)
+    int k0 = __reduce_add_sync(FULLMASK, (lane < rank ? cta.x : 0) + (lane < warp ? s_free[lane] : 0));
     const bool ok = taken <= free_pages && over == 0 && bad == 0;
     if (ok && k0 < taken) {
         // the k-th free page belongs to the last sequence whose place is at or before k
@@ -255,22 +248,23 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
             *a.n_copies = ok ? (int)(base >> 40) : 0;
         }
     }
-    if (nc > 1) cluster.barrier_wait();  // no CTA leaves while another may read its shared memory
 }
 
 // Compaction: used pages at or above the number of used pages go to the free pages below
 // it, the k-th to the k-th.
-__global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(const PagesArgs a)
+__global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(const __grid_constant__ PagesArgs a)
 {
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ int s_used[PG_WARPS], s_mv[PG_SLICES], s_ho[PG_SLICES], s_cut[2];
-    __shared__ unsigned long long s_sh[PG_WARPS + 1];
+    __shared__ unsigned long long s_sh[2][PG_WARPS];
     const int rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gw = rank * PG_WARPS + warp, gt = rank * PG_THREADS + tid;
     const int per = (a.n_pages + PG_SLICES - 1) / PG_SLICES;
     const int64_t lo = (int64_t)gw * per;
     const int n_slice = (int)max((int64_t)0, min((int64_t)per, a.n_pages - lo));
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    touch_params(a);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     int n = 0;
     for (int i = lane; i < n_slice; i += 32) n += a.refs_in[lo + i] > 0;
@@ -280,7 +274,7 @@ __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS,
     cluster.sync();
     unsigned long long sum;
     const int mine = tid < PG_SLICES ? *cluster.map_shared_rank(&s_used[tid % PG_WARPS], tid / PG_WARPS) : 0;
-    pg_scan(mine, &sum, s_sh);
+    pg_scan(mine, &sum, s_sh[0]);
     const int used = (int)sum;
     // pages to move and holes of every slice; the one that holds the border is counted again
     const int cut = used / per;  // its slice (every page used: none)
@@ -301,7 +295,7 @@ __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS,
             holes = (int)max((int64_t)0, min((int64_t)per, (int64_t)a.n_pages - (int64_t)tid * per)) - mine;
         }
     }
-    const unsigned long long before = pg_scan((unsigned long long)holes << 32 | (unsigned)moves, &sum, s_sh);
+    const unsigned long long before = pg_scan((unsigned long long)holes << 32 | (unsigned)moves, &sum, s_sh[1]);
     const int total = (int)(uint32_t)sum;
     if (tid < PG_SLICES) {
         s_mv[tid] = (int)(uint32_t)before;
@@ -340,32 +334,26 @@ __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_THREADS,
 
 // One chunk of a page: the first `fill` positions of its segments.
 template <class V>
-__device__ __forceinline__ void copy_chunk(const PoolArg &q, int from, int to, int fill, int chunk)
+__device__ __forceinline__ void copy_chunk(const PoolArg &q, const char *src, char *dst, int fill, int chunk)
 {
     const uint32_t cols = (uint32_t)fill * q.token_vecs, all = cols * (uint32_t)q.segs;
-    const char *src = q.data + (int64_t)from * q.page_stride;
-    char *dst = q.data + (int64_t)to * q.page_stride;
+    auto place = [&](uint32_t c) {
+        if (q.segs == 1) return (int64_t)c * (int64_t)sizeof(V);
+        const uint32_t seg = c / cols;
+        return (int64_t)seg * q.seg_stride + (int64_t)(c - seg * cols) * (int64_t)sizeof(V);
+    };
     const uint32_t c0 = (uint32_t)chunk * (PC_THREADS * PC_VECS) + threadIdx.x;
     V v[PC_VECS];
-    int64_t off[PC_VECS];
-#pragma unroll
-    for (int i = 0; i < PC_VECS; i++) {
-        const uint32_t c = c0 + i * PC_THREADS;
-        if (c < all) {
-            const uint32_t seg = c / cols;
-            off[i] = (int64_t)seg * q.seg_stride + (int64_t)(c - seg * cols) * (int64_t)sizeof(V);
-            v[i] = *(const V *)(src + off[i]);
-        }
-    }
 #pragma unroll
     for (int i = 0; i < PC_VECS; i++)
-        if (c0 + i * PC_THREADS < all) *(V *)(dst + off[i]) = v[i];
+        if (c0 + i * PC_THREADS < all) v[i] = *(const V *)(src + place(c0 + i * PC_THREADS));
+#pragma unroll
+    for (int i = 0; i < PC_VECS; i++)
+        if (c0 + i * PC_THREADS < all) *(V *)(dst + place(c0 + i * PC_THREADS)) = v[i];
 }
 
-// The listed pages' contents, pool by pool: a fork copies the filled positions of its
-// copies, a compaction whole pages (and renames the tables' entries).
 template <bool FORK>
-__global__ void __launch_bounds__(PC_THREADS) pages_copy_kernel(const __grid_constant__ PagesArgs a, const __grid_constant__ PoolArgs pools)
+__global__ void __launch_bounds__(PC_THREADS, PC_CTAS) pages_copy_kernel(const __grid_constant__ PagesArgs a, const __grid_constant__ PoolArgs pools)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -389,29 +377,76 @@ __global__ void __launch_bounds__(PC_THREADS) pages_copy_kernel(const __grid_con
             if (bad) atomicAdd(&a.result[3], bad);
         }
     }
-    const int n = FORK ? *a.n_copies : a.result[1];
-    const int64_t units = (int64_t)n * pools.n * pools.chunks;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int chunk = (int)(u % pools.chunks);
-        const int64_t rest = u / pools.chunks;
-        const PoolArg &q = pools.p[rest % pools.n];
-        const int64_t k = rest / pools.n;
+    if (pools.n == 0) return;
+    const int n = FORK ? __ldcg(a.n_copies) : __ldcg(a.result + 1);
+    // work item (k-th copy, pool, chunk), the CTAs' steps carried from digit to digit
+    const int step_chunk = (int)(gridDim.x % (unsigned)pools.chunks), step_rest = (int)(gridDim.x / (unsigned)pools.chunks);
+    const int step_pool = step_rest % pools.n, step_k = step_rest / pools.n;
+    int chunk = (int)(blockIdx.x % (unsigned)pools.chunks), rest = (int)(blockIdx.x / (unsigned)pools.chunks);
+    int pool = rest % pools.n, k = rest / pools.n;
+    while (k < n) {
         int from, to, fill;
         if constexpr (FORK) {
             const int4 c = __ldcg(a.copies + k);
             from = c.x, to = c.y, fill = c.z;
         } else {
-            from = __ldcg(a.moves + 2 * k), to = __ldcg(a.moves + 2 * k + 1), fill = a.page_tokens;
+            const int2 c = __ldcg((const int2 *)a.moves + k);
+            from = c.x, to = c.y, fill = a.page_tokens;
         }
-        if (q.width == 16) copy_chunk<uint4>(q, from, to, fill, chunk);
-        else if (q.width == 4) copy_chunk<uint32_t>(q, from, to, fill, chunk);
-        else copy_chunk<uint8_t>(q, from, to, fill, chunk);
+        const PoolArg &q = pools.p[pool];
+        const char *src = q.data + (int64_t)from * q.page_stride;
+        char *dst = q.data + (int64_t)to * q.page_stride;
+        if (q.width == 16) copy_chunk<uint4>(q, src, dst, fill, chunk);
+        else if (q.width == 4) copy_chunk<uint32_t>(q, src, dst, fill, chunk);
+        else copy_chunk<uint8_t>(q, src, dst, fill, chunk);
+        chunk += step_chunk;
+        pool += step_pool;
+        k += step_k;
+        if (chunk >= pools.chunks) {
+            chunk -= pools.chunks;
+            pool++;
+        }
+        if (pool >= pools.n) {
+            pool -= pools.n;
+            k++;
+        }
     }
+}
+
+// The deciding kernels: one cluster, a programmatic dependent of what runs before.
+static cudaError_t launch_cluster(void (*kernel)(PagesArgs), int ctas, int smem, const PagesArgs &a, cudaStream_t s)
+{
+    static bool ready[2][MAX_DEVICES] = {};
+    const int dev = current_device();
+    if (dev < 0 || dev >= MAX_DEVICES) return cudaErrorInvalidDevice;
+    bool &done = ready[kernel == pages_fork_kernel][dev];
+    if (!done) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess && kernel == pages_fork_kernel)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     pages_fork_smem(G4S_PAGES_MAX_SEQS, G4S_PAGES_MAX_SEQS));
+        if (e != cudaSuccess) return e;
+        done = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(PG_THREADS);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)ctas;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 int pages_chunk_vecs() { return PC_THREADS * PC_VECS; }
 
-int pages_fork_smem(int n_in, int n_out) { return 5 * (n_in > n_out ? n_in : n_out) * (int)sizeof(int); }
+int pages_fork_smem(int n_in, int n_out) { return 6 * (n_in > n_out ? n_in : n_out) * (int)sizeof(int); }
 
 template <bool FORK>
 static cudaError_t launch_copy(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s)
@@ -419,50 +454,22 @@ static cudaError_t launch_copy(const PagesArgs &a, const PoolArgs &pools, int sm
     int64_t work = (int64_t)a.max_copies * pools.n * pools.chunks;
     if (!FORK && work < a.n_in) work = a.n_in;
     if (work == 0) return cudaSuccess;
-    const int64_t most = (int64_t)sms * 8;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(work < most ? work : most));
-    cfg.blockDim = dim3(PC_THREADS);
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, pages_copy_kernel<FORK>, a, pools);
+    const int64_t most = (int64_t)sms * PC_CTAS;
+    return launch_dependent(pages_copy_kernel<FORK>, work < most ? work : most, PC_THREADS, 0, s, a, pools);
 }
 
 cudaError_t launch_pages_fork(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s)
 {
-    const int smem = pages_fork_smem(a.n_in, a.n_out);
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(pages_fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return e;
-    }
     // one CTA for few pages and table entries: its barriers are cheaper than the cluster's
-    const int nc = a.n_pages <= PG_ONE_PAGES && (int64_t)a.n_in * a.width <= PG_ONE_ENTRIES ? 1 : PG_CLUSTER;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)nc);
-    cfg.blockDim = dim3(PG_THREADS);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)nc;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, pages_fork_kernel, a);
+    const bool one = a.n_pages <= PG_ONE_PAGES && (int64_t)a.n_in * a.width <= PG_ONE_ENTRIES;
+    const cudaError_t e = launch_cluster(pages_fork_kernel, one ? 1 : PG_CLUSTER, pages_fork_smem(a.n_in, a.n_out), a, s);
     if (e != cudaSuccess || a.n_new == 0) return e;
     return launch_copy<true>(a, pools, sms, s);
 }
 
 cudaError_t launch_pages_compact(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s)
 {
-    pages_compact_kernel<<<PG_CLUSTER, PG_THREADS, 0, s>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_cluster(pages_compact_kernel, PG_CLUSTER, 0, a, s);
     if (e != cudaSuccess) return e;
     return launch_copy<false>(a, pools, sms, s);
 }

@@ -537,7 +537,8 @@ int32_t g4s_pages_fork(g4s_ctx *ctx, const g4s_page_cache *cache, int32_t n_in, 
  * lens is only read (in->lens).
  *   page_map  [n_pages] the new id of each page, -1 for a free one (for holders
  *             besides the tables)
- *   moves     [n_pages] (from, to) pairs; only the moved ones are written
+ *   moves     [n_pages] (from, to) pairs, 8-byte aligned; only the moved ones
+ *             are written
  *   result    int32 [4]: pages used; pages moved; 0; bad inputs (lengths out
  *             of range, taken as the nearest in range; table entries outside the
  *             pool, kept; entries of a free page, set to -1)
