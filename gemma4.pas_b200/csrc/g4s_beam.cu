@@ -535,35 +535,43 @@ __device__ __forceinline__ bool beam_before(const ulonglong2 &x, const ulonglong
     return (x.x > y.x) | ((x.x == y.x) & (x.y > y.y));  // (no branch)
 }
 
-// The first N of n entries (rank, tie) in shared memory, in order, to out; rest(tie) for
-// each of the others.  Up to 512 entries every one counts those before it, a warp four
-// entries at a time; more are sorted in place (padded with zeros to P, a power of two).
+// E entries from e0 on of n (rank, tie): each one's place by the entries before it.
+template <int E, class Put, class Rest>
+__device__ __forceinline__ void beam_places(const ulonglong2 *v, int e0, int n, int N, Put &put, Rest &rest)
+{
+    const int lane = threadIdx.x & 31;
+    ulonglong2 x[E];
+    int before[E] = {};
+#pragma unroll
+    for (int k = 0; k < E; k++) x[k] = v[e0 + k];  // (zeros from n on)
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const ulonglong2 y = v[min(i0 + lane, n)];
+#pragma unroll
+        for (int k = 0; k < E; k++) before[k] += __popc(__ballot_sync(FULLMASK, beam_before(y, x[k])));
+    }
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+        if (lane == k && x[k].y) {
+            if (before[k] < N) put(before[k], x[k]);
+            else rest(x[k].y);
+        }
+    }
+}
+
+// The first N of n entries (rank, tie) in shared memory, in order: put(place, entry) for
+// each of them, rest(tie) for each of the others.  Up to 512 entries every one counts those
+// before it, a warp one entry at a time, or four (over 64 entries the loads from shared
+// memory bound it); more are sorted in place (padded with zeros to P, a power of two).
 // Pairs closer than 64 places stay within a warp's 32 exchanges, so only the wider steps
 // need the CTA.
-template <class Rest>
-__device__ __forceinline__ void beam_first(ulonglong2 *v, int n, int P, int N, ulonglong2 *out, Rest rest)
+template <class Put, class Rest>
+__device__ __forceinline__ void beam_first(ulonglong2 *v, int n, int P, int N, Put put, Rest rest)
 {
-    const int tid = threadIdx.x, lane = tid & 31;
-    if (n <= 512) {
-        for (int e0 = tid / 32 * 4; e0 < n; e0 += BC_WARPS * 4) {
-            ulonglong2 x[4];
-            int before[4] = {};
-#pragma unroll
-            for (int k = 0; k < 4; k++) x[k] = v[e0 + k];  // (zeros from n on)
-            for (int i = lane; i < n; i += 32) {
-                const ulonglong2 y = v[i];
-#pragma unroll
-                for (int k = 0; k < 4; k++) before[k] += beam_before(y, x[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int c = __reduce_add_sync(FULLMASK, before[k]);
-                if (x[k].y && lane == k) {
-                    if (c < N) out[c] = x[k];
-                    else rest(x[k].y);
-                }
-            }
-        }
+    const int tid = threadIdx.x;
+    if (n <= 64) {
+        for (int e = tid / 32; e < n; e += BC_WARPS) beam_places<1>(v, e, n, N, put, rest);
+    } else if (n <= 512) {
+        for (int e = tid / 32 * 4; e < n; e += BC_WARPS * 4) beam_places<4>(v, e, n, N, put, rest);
     } else {
         for (int k = 2; k <= P; k <<= 1) {
             for (int j = k >> 1; j > 0; j >>= 1) {
@@ -583,19 +591,24 @@ __device__ __forceinline__ void beam_first(ulonglong2 *v, int n, int P, int N, u
         __syncthreads();
         for (int e = tid; e < n; e += BC_THREADS) {
             if (v[e].y == 0) continue;
-            if (e < N) out[e] = v[e];
+            if (e < N) put(e, v[e]);
             else rest(v[e].y);
         }
     }
     __syncthreads();
 }
 
-// The smallest logit with at least this key (NaN, which no logit reaches, above the
-// largest finite one's, which +inf has too).
+// The smallest logit of the type with at least this key (NaN, which no logit reaches, above
+// the largest finite one's, which +inf has too).
 template <int DT>
 __device__ __forceinline__ float beam_floor(uint32_t key)
 {
-    return key > f2key(beam_max<DT>()) ? __uint_as_float(0x7fc00000u) : key2f(key);
+    if (key > f2key(beam_max<DT>())) return __uint_as_float(0x7fc00000u);
+    if (DT == G4S_BF16) {  // keys of bf16 numbers end in 0000 (from +0 on) or ffff
+        const uint32_t low = key & 0x80000000u ? 0u : 0xffffu;
+        if ((key & 0xffffu) != low) key = key & 0x80000000u ? (key | 0xffffu) + 1u : key | 0xffffu;
+    }
+    return key2f(key);
 }
 constexpr uint32_t BEAM_KEY_MIN = 0xeb60d36u;  // the key after -1e30's
 
@@ -612,19 +625,37 @@ __device__ __forceinline__ uint32_t unit_mask(const char *p, int n, int lane, fl
         for (int j = 0; j < BNV; j++) r[j] = __ldg((const uint4 *)p + j * 32 + lane);
 #pragma unroll
         for (int j = 0; j < BNV; j++) {
-            float v[T::VW];
-            T::unpack(r[j], v);
+            const uint32_t w[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
 #pragma unroll
-            for (int k = 0; k < T::VW; k++) m |= (v[k] >= x ? 1u : 0u) << (j * T::VW + k);
+            for (int k = 0; k < 4; k++) {
+                uint32_t ge;
+                if constexpr (DT == G4S_BF16) {  // both halves at once; x is a bf16 (or NaN) here
+                    const uint32_t x2 = __byte_perm(__float_as_uint(x), 0u, 0x3232);
+                    asm("set.ge.u32.bf16x2 %0, %1, %2;" : "=r"(ge) : "r"(w[k]), "r"(x2));
+                    m |= ge & (0x00010001u << (j * 4 + k));
+                } else {
+                    asm("set.ge.u32.f32 %0, %1, %2;" : "=r"(ge) : "f"(__uint_as_float(w[k])), "f"(x));
+                    m |= ge & (1u << (j * 4 + k));
+                }
+            }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < BeamGeo<DT>::EPL; i++) {
-            const int e = ((i / T::VW) * 32 + lane) * T::VW + i % T::VW;
-            if (e < n && T::load1(p, e) >= x) m |= 1u << i;
-        }
+        for (int j = 0; j < BNV; j++)
+#pragma unroll
+            for (int k = 0; k < T::VW; k++) {
+                const int e = (j * 32 + lane) * T::VW + k, bit = DT == G4S_BF16 ? j * 4 + k / 2 + (k & 1) * 16 : j * 4 + k;
+                if (e < n && T::load1(p, e) >= x) m |= 1u << bit;
+            }
     }
     return m;
+}
+// The unit position of a bit of the mask (bf16: the words' lower halves, then the upper).
+template <int DT>
+__device__ __forceinline__ int mask_place(int bit, int lane)
+{
+    if (DT == G4S_F32) return ((bit >> 2) * 32 + lane) * 4 + (bit & 3);
+    return (((bit & 15) >> 2) * 32 + lane) * 8 + (bit & 3) * 2 + (bit >> 4);
 }
 
 template <int DT, bool VEC>
@@ -635,30 +666,37 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
     const float NEG_INF = -__uint_as_float(0x7f800000u);
     extern __shared__ ulonglong2 s_mem[];
     ulonglong2 *ent = s_mem;                         // [pe] the beams' items: (rank, tie), rank 0: none
-    ulonglong2 *cand = ent + a.pe;                   // [pc] collected tokens
+    ulonglong2 *list = ent + a.pe;                   // [pe] those that can be among the first
+    ulonglong2 *cand = list + a.pe;                  // [pc] collected tokens
     ulonglong2 *first = cand + a.pc;                 // [n_out] the first in order
     __shared__ BeamRow s_row[G4S_BEAM_MAX];
     __shared__ int s_sel[G4S_BEAM_MAX];      // items of the row among the first
     __shared__ uint32_t s_least[G4S_BEAM_MAX];  // the least key of its tokens wanted
-    __shared__ int s_m;
+    __shared__ int s_m, s_items, s_n;
+    __shared__ uint32_t s_bound;             // upper half of a rank that N items reach
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int W = a.beams, N = a.n_out, row0 = (int)blockIdx.x * W;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    for (int e = tid; e < a.pe + a.pc + N; e += BC_THREADS) s_mem[e] = make_ulonglong2(0, 0);
+    for (int e = tid; e < 2 * a.pe + a.pc + N; e += BC_THREADS) s_mem[e] = make_ulonglong2(0, 0);
     if (tid < G4S_BEAM_MAX) {
         s_least[tid] = BEAM_KEY_MIN;
         s_sel[tid] = 0;
     }
-    if (tid == 0) s_m = 0;
+    if (tid == 0) {
+        s_m = s_items = s_n = 0;
+        s_bound = 0;
+    }
     touch_params(a);
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // 1. two warps a beam: one sums the row, the other takes its n_out largest items
-    for (int task = warp; task < 2 * W; task += BC_WARPS) {
-        const bool sums = task < W;
-        const int w = sums ? task : task - W, row = row0 + w;
+    // 1. two warps a beam (one from 16 beams on): one sums the row, the other takes its
+    // n_out largest items and then ranks them
+    const bool pairs = W < 16, scaled = a.alpha2[0] != 0.0f;
+    if (warp < (pairs ? 2 * W : W)) {
+        const bool sums = !pairs || warp < W, takes = !pairs || warp >= W;
+        const int w = warp < W ? warp : warp - W, row = row0 + w;
         const float4 *st = a.istat + (int64_t)row * a.ipr;
         float4 q[BIPL];  // (a dead row's are what an earlier call left, and are not used)
 #pragma unroll
@@ -705,16 +743,21 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
                 r.inv = pair_exp(pair_mul(ln, Pair{-a.alpha2[0], -a.alpha2[1]}));
             }
             if (lane == 0) s_row[w] = r;
-        } else if (kind == BEAM_DONE) {
+            __syncwarp();
+            if (pairs) asm volatile("bar.arrive %0, 64;" ::"r"(1 + w) : "memory");
+        }
+        int cnt = 0;
+        if (takes && kind == BEAM_DONE) {
             if (lane == 0) ent[w * N].y = beam_tie(w, 0u, 0u);
-        } else if (live) {
+            cnt = 1;
+        } else if (takes && live) {
             auto full = [](uint32_t k) { return SH ? (k << SH) | (k & 0x8000u ? 0u : 0xffffu) : k; };
             int nv = 0;
 #pragma unroll
             for (int j = 0; j < BIPL; j++) nv += __popc(__ballot_sync(FULLMASK, key[j] != 0));
             // the largest `above` with at least N items at or above it, between the least of
             // the lanes' largest (for N <= 32) and the largest; out early at N exactly
-            const int cnt = min(N, nv);
+            cnt = min(N, nv);
             uint32_t above = 0;  // keys over it are taken, then those equal to it
             if (nv > N) {
                 uint32_t lo = max(N <= 32 ? __reduce_min_sync(FULLMASK, kmax) : 0u, 1u), hi = best;
@@ -753,30 +796,45 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
             const float ref = key2f(full(best));
             for (int i = lane; i < cnt; i += 32) ent[w * N + i].x = pair_bits(beam_x(a, ref, tie_key(ent[w * N + i].y)));
         }
-    }
-    __syncthreads();
-
-    // 2. the items by their best token
-    const bool scaled = a.alpha2[0] != 0.0f;
-    for (int e = tid; e < W * N; e += BC_THREADS) {
-        const ulonglong2 v = ent[e];
-        if (v.y) {
-            const BeamRow &r = s_row[tie_beam(v.y)];
-            ent[e].x = beam_rank(r, beam_score(r, bits_pair(v.x)), scaled);
+        if (takes) {
+            if (pairs) asm volatile("bar.sync %0, 64;" ::"r"(1 + w) : "memory");
+            else __syncwarp();
+            const BeamRow &r = s_row[w];
+            uint32_t low = 0xffffffffu;
+            for (int i = lane; i < cnt; i += 32) {
+                const uint64_t rank = beam_rank(r, beam_score(r, bits_pair(ent[w * N + i].x)), scaled);
+                ent[w * N + i].x = rank;
+                low = min(low, (uint32_t)(rank >> 32));
+            }
+            low = __reduce_min_sync(FULLMASK, low);
+            if (lane == 0) {
+                atomicAdd(&s_items, cnt);
+                if (cnt == N) atomicMax(&s_bound, low);
+            }
         }
     }
     __syncthreads();
-    // a beam's tokens count from its best item left out; where all of its N items are
-    // in, from the last of them; where it has no more, all
-    beam_first(ent, W * N, a.pe, N, first, [&](uint64_t tie) { atomicMax(&s_least[tie_beam(tie)], tie_key(tie)); });
-    const bool chosen = tid < N && first[tid].y;
-    if (chosen) atomicAdd(&s_sel[tie_beam(first[tid].y)], 1);
-    const int nsel = __syncthreads_count(chosen);
-    if (tid == 0 && nsel == N) {
-        const uint64_t t = first[N - 1].y;
-        if (s_sel[tie_beam(t)] == N) s_least[tie_beam(t)] = max(tie_key(t), BEAM_KEY_MIN);
+
+    // 2. the items by their best token; below the best beam's last one they are out at once
+    auto out = [&](uint64_t tie) { atomicMax(&s_least[tie_beam(tie)], tie_key(tie)); };
+    for (int e = tid; e < W * N; e += BC_THREADS) {
+        const ulonglong2 x = ent[e];
+        if (x.y == 0) continue;
+        if ((uint32_t)(x.x >> 32) >= s_bound) list[atomicAdd(&s_n, 1)] = x;
+        else out(x.y);
     }
     __syncthreads();
+    beam_first(
+        list, s_n, a.pe, N,
+        [&](int at, const ulonglong2 &x) {
+            first[at] = x;
+            atomicAdd(&s_sel[tie_beam(x.y)], 1);
+        },
+        out);
+    const int nsel = min(N, s_items);
+    // a beam's tokens count from its best item left out; where all of its N items are
+    // in, from the last of them; where it has no more, all
+    auto least = [&](int w) { return s_sel[w] == N ? max(tie_key(first[N - 1].y), BEAM_KEY_MIN) : s_least[w]; };
 
     // 3. their tokens, a warp a unit.  Where they are more than fit (equal logits, a small
     // vocabulary), again item by item: only n_out - j of the item in place j can count (the
@@ -785,7 +843,6 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
         const int o = atomicAdd(&s_m, 1);
         if (o < a.pc) cand[o] = make_ulonglong2(0, beam_tie(w, key, (uint32_t)id));
     };
-    auto place = [&](int i) { return ((i / T::VW) * 32 + lane) * T::VW + i % T::VW; };
     for (int task = warp; task < nsel * a.upi; task += BC_WARPS) {
         const uint64_t t = first[task / a.upi].y;
         const int w = tie_beam(t), u = task % a.upi;
@@ -797,8 +854,8 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
         const int n = (int)min((int64_t)UNIT, a.vocab - e0);
         if (n <= 0) continue;
         const char *p = (const char *)a.logits + ((int64_t)(row0 + w) * a.row_stride + e0) * T::ESIZE;
-        for (uint32_t m = unit_mask<DT, VEC>(p, n, lane, beam_floor<DT>(s_least[w])); m; m &= m - 1) {
-            const int e = place(__ffs(m) - 1);
+        for (uint32_t m = unit_mask<DT, VEC>(p, n, lane, beam_floor<DT>(least(w))); m; m &= m - 1) {
+            const int e = mask_place<DT>(__ffs(m) - 1, lane);
             push(w, beam_key<DT>(T::load1(p, e)), e0 + e);
         }
     }
@@ -826,13 +883,13 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
                     const char *pu = p + (int64_t)u * T::ESIZE;
                     uint32_t m = unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(key));
                     if (but) m &= ~unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(but));
-                    for (; upto < n && m; m &= m - 1) c += u + place(__ffs(m) - 1) <= upto;
+                    for (; upto < n && m; m &= m - 1) c += u + mask_place<DT>(__ffs(m) - 1, lane) <= upto;
                     c += __popc(m);
                 }
                 return (int)__reduce_add_sync(FULLMASK, c);
             };
             // the quota-th largest key, and the place up to which its equals are taken
-            uint32_t lo = s_least[w], hi = tie_key(t);
+            uint32_t lo = least(w), hi = tie_key(t);
             int last = n;
             if (count(lo, 0u, n) > quota) {
                 while (lo < hi) {
@@ -852,7 +909,7 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
             for (int u = 0; u < n; u += UNIT) {
                 const char *pu = p + (int64_t)u * T::ESIZE;
                 for (uint32_t m = unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(lo)); m; m &= m - 1) {
-                    const int e = place(__ffs(m) - 1);
+                    const int e = mask_place<DT>(__ffs(m) - 1, lane);
                     const uint32_t key = beam_key<DT>(T::load1(pu, e));
                     if (key > lo || u + e <= last) push(w, key, e0 + u + e);
                 }
@@ -866,9 +923,9 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
         const BeamRow &r = s_row[tie_beam(t)];
         cand[e].x = beam_rank(r, beam_score(r, beam_x(a, r.ref, tie_key(t))), scaled);
     }
-    if (tid < N) first[tid] = make_ulonglong2(0, 0);
     __syncthreads();
-    beam_first(cand, m, a.pc, N, first, [](uint64_t) {});
+    beam_first(
+        cand, m, a.pc, N, [&](int at, const ulonglong2 &x) { first[at] = x; }, [](uint64_t) {});
     if (tid < N) {
         const int64_t o = (int64_t)blockIdx.x * N + tid;
         float score = NEG_INF;
@@ -921,7 +978,7 @@ static cudaError_t launch_beam_t(BeamArgs &a, int sms, cudaStream_t s)
     const int64_t items = (int64_t)a.rows * a.ipr, blocks = (items + per - 1) / per;
     e = launch_dependent(beam_stream_kernel<DT, VEC, CAP>, blocks < most ? blocks : most, BS_THREADS, 0, s, a);
     if (e != cudaSuccess) return e;
-    return launch_dependent(beam_combine_kernel<DT, VEC>, a.rows / a.beams, BC_THREADS, (size_t)(a.pe + a.pc + a.n_out) * 16, s, a);
+    return launch_dependent(beam_combine_kernel<DT, VEC>, a.rows / a.beams, BC_THREADS, (size_t)(2 * a.pe + a.pc + a.n_out) * 16, s, a);
 }
 
 // tanh(q) / q = 1 + q^2 P(q^2) on |q| <= 1/2, P of degree 3 fitted for the least largest

@@ -994,9 +994,14 @@ __global__ void __launch_bounds__(COMBINE_THREADS) full_combine_kernel(SampleArg
     const int t = threadIdx.x;
     const int row = blockIdx.x;
     const g4s_params p = a.params.get(row);
-    if (!(p.top_k <= 0 || p.top_k >= a.vocab)) return;  // uniform over the CTA
-    // resolve mode: only the draws the merge assigned to this shard
-    if (a.shard_mode == 2 && (!(p.temperature > 0.0f) || a.shard_tgt[row].w != a.shard_rank)) return;
+    // uniform over the CTA; resolve mode: only the draws the merge assigned to this shard
+    if (!(p.top_k <= 0 || p.top_k >= a.vocab) ||
+        (a.shard_mode == 2 && (!(p.temperature > 0.0f) || a.shard_tgt[row].w != a.shard_rank))) {
+        // a CTA without work waits too: a programmatic dependent of this grid takes its end
+        // as the end of everything before it
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     const SParams sp = make_sparams(a, p, row);
     const int ipr = (a.vocab + ITEM - 1) / ITEM;
     const float4 *st = a.istat + (int64_t)row * ipr;

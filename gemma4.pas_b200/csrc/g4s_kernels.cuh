@@ -237,7 +237,7 @@ inline cudaError_t launch_dependent(void (*kernel)(P...), int64_t blocks, int th
 }
 
 constexpr int BEAM_MAX_ITEMS = 128;  // items a row in the selection's statistics
-constexpr int BEAM_COMBINE_SMEM_MAX = (2048 + 4096 + 64) * 16;  // 32 beams, 64 continuations
+constexpr int BEAM_COMBINE_SMEM_MAX = (2 * 2048 + 4096 + 64) * 16;  // 32 beams, 64 continuations
 constexpr int BEAM_H1 = 5, BEAM_H2 = 8;  // coefficients of the folded softcap polynomials
 
 struct BeamArgs {
