@@ -75,30 +75,22 @@ __device__ __forceinline__ float beam_soft(float v, const BeamArgs &a)
     return __fmul_rn(aq <= 1.0f ? tanh_poly(q) : copysignf(w, q), a.softcap);
 }
 
-// One unit's vectors of this lane: logit (j, k) is unit position (j * 32 + lane) * VW + k.
-// Rows that are not 16-byte aligned are gathered element by element into the same places,
-// so that a row's sums do not depend on its alignment.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_unit(const char *p, int lane, uint4 (&r)[BS_NV])
+// A load of a row that no vector load fits: every 32nd logit (pair of words for bf16).
+template <int DT>
+__device__ __forceinline__ void load_single(const char *p, int lane, uint4 (&r)[BS_NV])
 {
-    using T = DtypeTraits<DT>;
+    uint32_t w[BS_NV * 4];
 #pragma unroll
-    for (int j = 0; j < BS_NV; j++) {
-        const int e0 = (j * 32 + lane) * T::VW;
-        if constexpr (VEC) {
-            r[j] = ld_stream_v4(p + (int64_t)e0 * T::ESIZE);
-        } else if constexpr (DT == G4S_F32) {
-            const float *f = (const float *)p + e0;
-            r[j] = make_uint4(__float_as_uint(__ldg(f)), __float_as_uint(__ldg(f + 1)), __float_as_uint(__ldg(f + 2)),
-                              __float_as_uint(__ldg(f + 3)));
+    for (int i = 0; i < BS_NV * 4; i++) {
+        if constexpr (DT == G4S_F32) {
+            w[i] = __float_as_uint(__ldg((const float *)p + i * 32 + lane));
         } else {
-            const unsigned short *h = (const unsigned short *)p + e0;
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) w[k] = (uint32_t)__ldg(h + 2 * k) | ((uint32_t)__ldg(h + 2 * k + 1) << 16);
-            r[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            const unsigned short *h = (const unsigned short *)p + i * 64 + lane;
+            w[i] = (uint32_t)__ldg(h) | ((uint32_t)__ldg(h + 32) << 16);
         }
     }
+#pragma unroll
+    for (int j = 0; j < BS_NV; j++) r[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
 }
 
 // Two fp32 numbers in a 64-bit register: the packed operations' operands.  two() is volatile
@@ -329,7 +321,7 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
             cp_async_wait<1>();
             ring_read<0>(at, r);
         } else if (whole) {
-            load_unit<DT, false>(cur.p, lane, r);
+            load_single<DT>(cur.p, lane, r);
         }
         float mx = NEG_INF;
         int way = 3;
@@ -612,8 +604,17 @@ __device__ __forceinline__ float beam_floor(uint32_t key)
 }
 constexpr uint32_t BEAM_KEY_MIN = 0xeb60d36u;  // the key after -1e30's
 
-// Which of the lane's logits of a unit (n left) are at or above x: bit j * VW + k for
-// logit (j, k).
+// The unit position of bit `bit` of a lane's mask: logit (j, k) at j * 4 + k (bf16: the words'
+// lower halves, then the upper); of rows that no vector load fits, every 32nd logit.
+template <int DT, bool VEC>
+__device__ __forceinline__ int mask_place(int bit, int lane)
+{
+    if (!VEC) return bit * 32 + lane;
+    if (DT == G4S_F32) return ((bit >> 2) * 32 + lane) * 4 + (bit & 3);
+    return (((bit & 15) >> 2) * 32 + lane) * 8 + (bit & 3) * 2 + (bit >> 4);
+}
+
+// Which of the lane's logits of a unit (n left) are at or above x.
 template <int DT, bool VEC>
 __device__ __forceinline__ uint32_t unit_mask(const char *p, int n, int lane, float x)
 {
@@ -640,22 +641,14 @@ __device__ __forceinline__ uint32_t unit_mask(const char *p, int n, int lane, fl
             }
         }
     } else {
+        float v[BeamGeo<DT>::EPL];
 #pragma unroll
-        for (int j = 0; j < BNV; j++)
+        for (int i = 0; i < BeamGeo<DT>::EPL; i++) v[i] = T::load1(p, min(mask_place<DT, VEC>(i, lane), n - 1));
 #pragma unroll
-            for (int k = 0; k < T::VW; k++) {
-                const int e = (j * 32 + lane) * T::VW + k, bit = DT == G4S_BF16 ? j * 4 + k / 2 + (k & 1) * 16 : j * 4 + k;
-                if (e < n && T::load1(p, e) >= x) m |= 1u << bit;
-            }
+        for (int i = 0; i < BeamGeo<DT>::EPL; i++)
+            m |= (mask_place<DT, VEC>(i, lane) < n && v[i] >= x ? 1u : 0u) << i;
     }
     return m;
-}
-// The unit position of a bit of the mask (bf16: the words' lower halves, then the upper).
-template <int DT>
-__device__ __forceinline__ int mask_place(int bit, int lane)
-{
-    if (DT == G4S_F32) return ((bit >> 2) * 32 + lane) * 4 + (bit & 3);
-    return (((bit & 15) >> 2) * 32 + lane) * 8 + (bit & 3) * 2 + (bit >> 4);
 }
 
 template <int DT, bool VEC>
@@ -855,7 +848,7 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
         if (n <= 0) continue;
         const char *p = (const char *)a.logits + ((int64_t)(row0 + w) * a.row_stride + e0) * T::ESIZE;
         for (uint32_t m = unit_mask<DT, VEC>(p, n, lane, beam_floor<DT>(least(w))); m; m &= m - 1) {
-            const int e = mask_place<DT>(__ffs(m) - 1, lane);
+            const int e = mask_place<DT, VEC>(__ffs(m) - 1, lane);
             push(w, beam_key<DT>(T::load1(p, e)), e0 + e);
         }
     }
@@ -883,7 +876,7 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
                     const char *pu = p + (int64_t)u * T::ESIZE;
                     uint32_t m = unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(key));
                     if (but) m &= ~unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(but));
-                    for (; upto < n && m; m &= m - 1) c += u + mask_place<DT>(__ffs(m) - 1, lane) <= upto;
+                    for (; upto < n && m; m &= m - 1) c += u + mask_place<DT, VEC>(__ffs(m) - 1, lane) <= upto;
                     c += __popc(m);
                 }
                 return (int)__reduce_add_sync(FULLMASK, c);
@@ -909,14 +902,14 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
             for (int u = 0; u < n; u += UNIT) {
                 const char *pu = p + (int64_t)u * T::ESIZE;
                 for (uint32_t m = unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(lo)); m; m &= m - 1) {
-                    const int e = mask_place<DT>(__ffs(m) - 1, lane);
+                    const int e = mask_place<DT, VEC>(__ffs(m) - 1, lane);
                     const uint32_t key = beam_key<DT>(T::load1(pu, e));
                     if (key > lo || u + e <= last) push(w, key, e0 + u + e);
                 }
             }
         }
         __syncthreads();
-        m = s_m;
+        m = min(s_m, a.pc);  // (never more, unless the logits changed since the streaming pass)
     }
     for (int e = tid; e < m; e += BC_THREADS) {
         const uint64_t t = cand[e].y;
