@@ -251,73 +251,60 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
 }
 
 // Compaction: used pages at or above the number of used pages go to the free pages below
-// it, the k-th to the k-th.
+// it, the k-th to the k-th.  A warp walks a slice of the pages; every CTA has every slice's
+// count in its shared memory.
 __global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(const __grid_constant__ PagesArgs a)
 {
     cg::cluster_group cluster = cg::this_cluster();
-    __shared__ int s_used[PG_WARPS], s_mv[PG_SLICES], s_ho[PG_SLICES], s_cut[2];
-    __shared__ unsigned long long s_sh[2][PG_WARPS];
-    const int rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int gw = rank * PG_WARPS + warp, gt = rank * PG_THREADS + tid;
-    const int per = (a.n_pages + PG_SLICES - 1) / PG_SLICES;
+    __shared__ int s_used[PG_SLICES];
+    const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int slices = nc * PG_WARPS, gw = rank * PG_WARPS + warp, gt = rank * PG_THREADS + tid;
+    const int per = (a.n_pages + slices - 1) / slices;
     const int64_t lo = (int64_t)gw * per;
     const int n_slice = (int)max((int64_t)0, min((int64_t)per, a.n_pages - lo));
+    auto sync = [&] {
+        if (nc > 1) cluster.sync();
+        else __syncthreads();
+    };
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     touch_params(a);
+    sync();  // (every CTA runs, before any writes to another's shared memory)
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     int n = 0;
+#pragma unroll 8
     for (int i = lane; i < n_slice; i += 32) n += a.refs_in[lo + i] > 0;
     n = __reduce_add_sync(FULLMASK, n);
-    if (lane == 0) s_used[warp] = n;
-    if (tid < 2) s_cut[tid] = 0;
-    cluster.sync();
-    unsigned long long sum;
-    const int mine = tid < PG_SLICES ? *cluster.map_shared_rank(&s_used[tid % PG_WARPS], tid / PG_WARPS) : 0;
-    pg_scan(mine, &sum, s_sh[0]);
-    const int used = (int)sum;
-    // pages to move and holes of every slice; the one that holds the border is counted again
-    const int cut = used / per;  // its slice (every page used: none)
-    for (int64_t p = (int64_t)cut * per + tid; p < min((int64_t)(cut + 1) * per, (int64_t)a.n_pages); p += PG_THREADS) {
-        const bool u = a.refs_in[p] > 0;
-        if (u && p >= used) atomicAdd(&s_cut[0], 1);
-        if (!u && p < used) atomicAdd(&s_cut[1], 1);
+    if (lane < nc) (nc > 1 ? cluster.map_shared_rank(s_used, lane) : s_used)[gw] = n;
+    sync();
+    // pages used, before this warp's slice, and below the border
+    int used = 0, before = 0, below = 0;
+    for (int i = lane; i < slices; i += 32) {
+        used += s_used[i];
+        before += i < gw ? s_used[i] : 0;
     }
-    __syncthreads();
-    int moves = 0, holes = 0;
-    if (tid < PG_SLICES) {
-        if (tid == cut) {
-            moves = s_cut[0];
-            holes = s_cut[1];
-        } else if (tid > cut) {
-            moves = mine;
-        } else {
-            holes = (int)max((int64_t)0, min((int64_t)per, (int64_t)a.n_pages - (int64_t)tid * per)) - mine;
-        }
-    }
-    const unsigned long long before = pg_scan((unsigned long long)holes << 32 | (unsigned)moves, &sum, s_sh[1]);
-    const int total = (int)(uint32_t)sum;
-    if (tid < PG_SLICES) {
-        s_mv[tid] = (int)(uint32_t)before;
-        s_ho[tid] = (int)(before >> 32);
-    }
-    __syncthreads();
-    int m0 = s_mv[gw], h0 = s_ho[gw];
+    used = __reduce_add_sync(FULLMASK, used);
+    before = __reduce_add_sync(FULLMASK, before);
+    const int cut = used / per;  // the slice that holds the border (every page used: none)
+    for (int i = lane; i < min(cut, slices); i += 32) below += s_used[i];
+    for (int64_t p = (int64_t)cut * per + lane; p < used; p += 32) below += a.refs_in[p] > 0;
+    below = __reduce_add_sync(FULLMASK, below);
     for (int i0 = 0; i0 < n_slice; i0 += 32) {
         const int p = (int)lo + i0 + lane;
         const bool in = i0 + lane < n_slice;
         const int refs = in ? a.refs_in[p] : 0;
-        const bool mv = in && refs > 0 && p >= used, hole = in && refs <= 0 && p < used;
-        const unsigned mb = __ballot_sync(FULLMASK, mv), hb = __ballot_sync(FULLMASK, hole);
-        if (mv) a.moves[2 * (m0 + __popc(mb & ((1u << lane) - 1)))] = p;
-        if (hole) a.moves[2 * (h0 + __popc(hb & ((1u << lane) - 1))) + 1] = p;
-        m0 += __popc(mb);
-        h0 += __popc(hb);
+        const unsigned b = __ballot_sync(FULLMASK, refs > 0);
+        const int u = before + __popc(b & ((1u << lane) - 1));  // used pages below p
+        before += __popc(b);
+        const bool mv = refs > 0 && p >= used, hole = in && refs <= 0 && p < used;
+        if (mv) a.moves[2 * (u - below)] = p;
+        if (hole) a.moves[2 * (p - u) + 1] = p;
         if (in && !mv) a.page_map[p] = refs > 0 ? p : -1;
         if (in && !mv && !hole) a.refs_out[p] = refs > 0 ? refs : 0;
     }
-    cluster.sync();  // the moves are listed
-    for (int k = gt; k < total; k += PG_CLUSTER * PG_THREADS) {
+    sync();  // the moves are listed
+    for (int k = gt; k < used - below; k += nc * PG_THREADS) {
         const int from = __ldcg(a.moves + 2 * k), to = __ldcg(a.moves + 2 * k + 1);
         const int refs = a.refs_in[from];
         a.page_map[from] = to;
@@ -326,7 +313,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(const __gr
     }
     if (gt == 0) {
         a.result[0] = used;
-        a.result[1] = total;
+        a.result[1] = used - below;
         a.result[2] = 0;
         a.result[3] = 0;
     }
@@ -469,7 +456,7 @@ cudaError_t launch_pages_fork(const PagesArgs &a, const PoolArgs &pools, int sms
 
 cudaError_t launch_pages_compact(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s)
 {
-    const cudaError_t e = launch_cluster(pages_compact_kernel, PG_CLUSTER, 0, a, s);
+    const cudaError_t e = launch_cluster(pages_compact_kernel, a.n_pages <= PG_ONE_PAGES ? 1 : PG_CLUSTER, 0, a, s);
     if (e != cudaSuccess) return e;
     return launch_copy<false>(a, pools, sms, s);
 }
