@@ -23,7 +23,7 @@ constexpr int PG_WARPS = PG_THREADS / 32;
 constexpr int PG_SLICES = PG_CLUSTER * PG_WARPS;  // a warp's slice of the page counts
 constexpr int PC_THREADS = 256;     // CTA of the copies
 constexpr int PC_VECS = 4;          // vectors a thread and step
-constexpr int PC_CTAS = 6;          // CTAs on an SM
+constexpr int PC_CTAS = 4;          // CTAs on an SM (2, 3, 5, 6, 8: slower)
 
 // Exclusive scan over the CTA's PG_THREADS values; *total gets the sum.  sh: PG_WARPS, not
 // written again before the next barrier.
