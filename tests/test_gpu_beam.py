@@ -447,3 +447,110 @@ def test_refusals(sampler, g4, torch_cuda):
         sampler.beam_reorder(P, 0, 4, [])
     torch_cuda.cuda.synchronize()
     assert ctypes.sizeof(g4.BeamParams) == 64
+
+
+def test_select_many_beams_with_length_penalty(sampler, g4, torch_cuda):
+    # one warp a beam from 16 beams on
+    rng = np.random.default_rng(12)
+    for W, N in ((15, 30), (16, 7), (17, 64), (31, 33)):
+        c = Case(torch_cuda, g4, logits(rng, 2 * W, 3000), "f32", W, N, alpha=0.9, done=rng.random(2 * W) < 0.2, T=0.8)
+        c.check(c.run(sampler))
+
+
+def test_select_rows_over_4_gib_apart(sampler, g4, torch_cuda):
+    torch = torch_cuda
+    rng = np.random.default_rng(13)
+    stride, V, W = 600_000_000, 5001, 4  # 2.4 GB a row: the last starts over 2^31 elements in
+    buf = torch.empty(5 * stride + V, device="cuda")
+    c = Case(torch, g4, logits(rng, 5, V), "f32", 5, 10)
+    for r in range(5):
+        buf[r * stride:r * stride + V] = c.buf.view(5, V)[r]
+    c.buf, c.ptr, c.stride = buf, buf.data_ptr(), stride
+    c.check(c.run(sampler))
+    del buf, c
+    torch.cuda.empty_cache()
+
+
+def test_select_two_contexts_at_once(g4, torch_cuda):
+    torch = torch_cuda
+    rng = np.random.default_rng(14)
+    with g4.Sampler(0, 64, 40000) as a, g4.Sampler(0, 64, 40000) as b:
+        ca = Case(torch, g4, logits(rng, 60, 33000), "f32", 6, 12)
+        cb = Case(torch, g4, logits(rng, 60, 33000), "bf16", 5, 5)
+        sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for s, c, st, dt in ((a, ca, sa, g4.F32), (b, cb, sb, g4.BF16)):
+                s.beam_select(c.ptr, dt, c.G, c.V, c.stride, c.cap, c.params, c.state(c.d), c.state(c.out[:3]),
+                              c.out[3].data_ptr(), c.out[4].data_ptr(), stream=st.cuda_stream)
+        torch.cuda.synchronize()
+        ca.check(ca.got())
+        cb.check(cb.got())
+
+
+def test_select_between_sampler_calls(sampler, g4, torch_cuda, oracle):
+    # the selection shares the context's item statistics with the full-vocabulary path, and starts behind it
+    torch = torch_cuda
+    rng = np.random.default_rng(15)
+    x = logits(rng, 8, 20000).astype(np.float32)
+    c = Case(torch, g4, x, "f32", 4, 4)
+    dx = torch.from_numpy(x).cuda()
+    u = torch.full((8,), 0.3, dtype=torch.float64, device="cuda")
+    tok = torch.zeros(8, dtype=torch.int32, device="cuda")
+    p = g4.make_params(1.0, 0, 0.95)
+    torch.cuda.synchronize()
+    sampler.sample(dx.data_ptr(), g4.F32, 8, 20000, 20000, p, 30.0, u.data_ptr(), tok.data_ptr())
+    torch.cuda.synchronize()
+    want = tok.cpu().numpy().copy()
+    first = c.run(sampler)
+    for _ in range(5):
+        tok.fill_(-1)
+        torch.cuda.synchronize()
+        sampler.sample(dx.data_ptr(), g4.F32, 8, 20000, 20000, p, 30.0, u.data_ptr(), tok.data_ptr())
+        sampler.beam_select(c.ptr, g4.F32, c.G, c.V, c.stride, c.cap, c.params, c.state(c.d), c.state(c.out[:3]),
+                            c.out[3].data_ptr(), c.out[4].data_ptr())
+        torch.cuda.synchronize()
+        assert np.array_equal(tok.cpu().numpy(), want)
+        assert all(np.array_equal(p, q) for p, q in zip(first, c.got()))
+    c.check(first)
+
+
+def test_select_on_the_lm_heads_logits(g4, torch_cuda, oracle):
+    """The LM head's logits (kept with out_logits) searched without leaving the device."""
+    torch = torch_cuda
+    rng = np.random.default_rng(16)
+    V, H, rows = 4096, 256, 8
+    blocks = rng.integers(0, 256, (V, H // 32, 18), dtype=np.uint8)
+    blocks[:, :, :2] = (rng.uniform(0.001, 0.02, (V, H // 32)).astype(np.float16)).view(np.uint8).reshape(V, H // 32, 2)
+    db = torch.from_numpy(blocks.reshape(-1).copy()).cuda()
+    nib = torch.zeros(V * H // 2, dtype=torch.uint8, device="cuda")
+    sc = torch.zeros(V * H // 32, dtype=torch.int16, device="cuda")
+    hidden = torch.from_numpy(rng.standard_normal((rows, H)).astype(np.float32)).cuda()
+    out = torch.zeros(rows, V, device="cuda")
+    tok = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    with g4.Sampler(0, rows, V) as s:
+        torch.cuda.synchronize()
+        g4.q4_repack(db.data_ptr(), V, H, nib.data_ptr(), sc.data_ptr())
+        torch.cuda.synchronize()
+        c = Case(torch, g4, np.zeros((rows, V)), "f32", 4, 8)
+        s.lmhead_sample(hidden.data_ptr(), rows, H, nib.data_ptr(), sc.data_ptr(), V, g4.make_params(0.0, 4, 1.0), 30.0, 0,
+                        tok.data_ptr(), logits_ptr=out.data_ptr())
+        c.ptr, c.stride = out.data_ptr(), V
+        got = c.run(s)
+        c.x = out.double().cpu().numpy()
+        c.check(got)
+
+
+def test_reorder_rows_over_4_gib_apart(sampler, g4, torch_cuda):
+    torch = torch_cuda
+    buf = torch.empty(3 * 2_200_000_000 + 64, dtype=torch.uint8, device="cuda")
+    row = 2_200_000_000
+    for r in range(3):
+        buf[r * row:r * row + 64] = r + 1
+    parents = torch.tensor([2, 0, 0], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    sampler.beam_reorder(parents.data_ptr(), 1, 3, [g4.BeamTensor(buf.data_ptr(), buf.data_ptr(), row, 2, 32, 1, 0, 32)])
+    torch.cuda.synchronize()
+    assert [int(buf[r * row + 63]) for r in range(3)] == [3, 1, 1]
+    del buf
+    torch.cuda.empty_cache()

@@ -420,3 +420,108 @@ def test_step_refusals(sampler, g4, torch_cuda):
     torch.cuda.synchronize()
     for a, b in zip(before, (s.scores, s.lens, s.refs, s.par)):
         assert torch.equal(a, b)  # nothing was launched
+
+
+def test_tables_without_pools(sampler, g4, torch_cuda):
+    rng = np.random.default_rng(20)
+    lens = rng.integers(0, 100, 9)
+    tables, refs, rest = scattered(rng, 9, lens, 8, 20, 300)
+    refs[rest[:40]] = 1
+    cache = Cache(torch_cuda, g4, rng, 300, 8, 20, layouts=())
+    run_fork(torch_cuda, g4, sampler, cache, tables, lens, refs, rng.integers(-1, 9, 12), 3)
+    run_compact(torch_cuda, g4, sampler, cache, tables, lens, refs, False)
+    run_fork(torch_cuda, g4, sampler, cache, np.full((0, 20), -1), [], refs, [-1, -1], 3)
+
+
+def test_pages_over_4_gib_in(g4, sampler, torch_cuda):
+    torch = torch_cuda
+    P, token, n_pages = 4, 1 << 18, 5000  # pages of 1 MiB
+    pool = torch.zeros(n_pages * P * token, dtype=torch.uint8, device="cuda")
+    page = pool.view(n_pages, P, token)
+    page[4990, :3] = 7
+    page[4991, :1] = 9
+    cache = g4.page_cache([g4.PagePool(pool.data_ptr(), P * token, 1, 0, token)], P, n_pages, 2)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    tables, lens = i32([[4990, -1], [4991, -1]]), i32([3, 1])
+    refs = torch.ones(n_pages, dtype=torch.int32, device="cuda")
+    refs[4999] = 0
+    ot, ol, orf, res = i32([[-9, -9], [-9, -9]]), i32([0, 0]), torch.zeros_like(refs), i32([0, 0, 0, 0])
+    src = i32([0, 0])
+    torch.cuda.synchronize()
+    sampler.pages_fork(cache, 2, tables.data_ptr(), lens.data_ptr(), refs.data_ptr(), 2, src.data_ptr(), 1, ot.data_ptr(),
+                       ol.data_ptr(), orf.data_ptr(), res.data_ptr())
+    torch.cuda.synchronize()
+    # the second sequence's page is freed: it is the lowest free one, and takes the copy
+    assert res.tolist() == [1, 0, 0, 0] and ot.tolist() == [[4991, -9], [4990, -9]] and ol.tolist() == [4, 4]
+    assert bool((page[4991, :3] == 7).all()) and bool((page[4991, 3] == 0).all())
+    del pool, page
+    torch.cuda.empty_cache()
+
+
+def test_fork_into_a_graph(sampler, g4, torch_cuda):
+    """A captured fork and compaction, replayed on other tables in the same memory."""
+    torch = torch_cuda
+    rng = np.random.default_rng(21)
+    n, P, width, n_pages = 6, 8, 12, 200
+    cache = Cache(torch, g4, rng, n_pages, P, width)
+    cu = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).cuda()
+    lens = rng.integers(1, 50, n)
+    tables, refs, _ = scattered(rng, n, lens, P, width, n_pages)
+    dt, dl, dr, ds = cu(tables), cu(lens), cu(refs), cu(np.zeros(n))
+    ot, ol, orf, res = cu(np.full((n, width), -9)), cu(np.zeros(n)), cu(np.zeros(n_pages)), cu(np.zeros(4))
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        sampler.pages_fork(cache.c, n, dt.data_ptr(), dl.data_ptr(), dr.data_ptr(), n, ds.data_ptr(), 2, ot.data_ptr(),
+                           ol.data_ptr(), orf.data_ptr(), res.data_ptr(), stream=stream.cuda_stream)
+    for k in range(4):
+        lens = rng.integers(0, 80, n)
+        tables, refs, _ = scattered(rng, n, lens, P, width, n_pages)
+        src = rng.integers(-1, n, n)
+        for d, h in ((dt, tables), (dl, lens), (dr, refs), (ds, src)):
+            d.copy_(cu(h))
+        for d, h in zip(cache.dev, cache.host):
+            d.copy_(torch.from_numpy(h))
+        ot.fill_(-9)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        wt, wl, wr, want, copies = beam_util.fork(tables, lens, refs, src, 2, P, width)
+        assert res.tolist() == want and np.array_equal(ot.cpu().numpy(), wt) and np.array_equal(ol.cpu().numpy(), wl)
+        assert np.array_equal(orf.cpu().numpy(), wr)
+        cache.check(copies)
+
+
+def test_fork_repeated_in_place_leaks_nothing(sampler, g4, torch_cuda):
+    """A long run of forks, growth, frees and compactions in place: the counts are what the tables hold."""
+    torch = torch_cuda
+    rng = np.random.default_rng(22)
+    n, P, width, n_pages = 12, 4, 40, 400
+    cache = Cache(torch, g4, rng, n_pages, P, width, layouts=((1, 16, 0, 0),))
+    cu = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).cuda()
+    tab = [cu(np.full((n, width), -1)), cu(np.full((n, width), -1))]
+    lens, refs, res = cu(np.zeros(n)), cu(np.zeros(n_pages)), cu(np.zeros(4))
+    mp, mv = cu(np.zeros(n_pages)), cu(np.zeros(n_pages))
+    for k in range(120):
+        a, b = tab[k % 2], tab[1 - k % 2]
+        src = np.arange(n) if k == 0 else rng.integers(0, n, n)
+        if k % 17 == 16:
+            src[rng.integers(0, n, 5)] = -1
+        ds = cu(src)
+        torch.cuda.synchronize()
+        sampler.pages_fork(cache.c, n, a.data_ptr(), lens.data_ptr(), refs.data_ptr(), n, ds.data_ptr(), int(rng.integers(0, 4)),
+                           b.data_ptr(), lens.data_ptr(), refs.data_ptr(), res.data_ptr())
+        if k % 10 == 9:
+            sampler.pages_compact(cache.c, n, b.data_ptr(), lens.data_ptr(), refs.data_ptr(), b.data_ptr(), refs.data_ptr(),
+                                  mp.data_ptr(), mv.data_ptr(), res.data_ptr())
+        torch.cuda.synchronize()
+        assert res.tolist()[3] == 0
+        L, T = lens.cpu().numpy(), b.cpu().numpy()
+        held = np.zeros(n_pages, np.int64)
+        for i in range(n):
+            np.add.at(held, T[i, :-(-int(L[i]) // P)], 1)
+        assert np.array_equal(held, refs.cpu().numpy()), k
+        if L.max() > width * P - 8:
+            lens.zero_()
+            refs.zero_()
