@@ -496,10 +496,10 @@ __device__ __forceinline__ Pair beam_x(const BeamArgs &a, float ref, uint32_t ke
     return fabsf(d.h) < 1e30f && fabsf(x) < 1e30f ? pair_mul(d, Pair{a.scale2[0], a.scale2[1]}) : Pair{x, 0.0f};
 }
 
-// A continuation's score from its x.
+// A continuation's score from its x (which a beam's score of 1e30 or more, or +inf, swallows).
 __device__ __forceinline__ Pair beam_score(const BeamRow &r, Pair x)
 {
-    if (r.kind == BEAM_DONE) return {r.score, 0.0f};
+    if (r.kind == BEAM_DONE || !(fabsf(r.score) < 1e30f)) return {r.score, 0.0f};
     return fabsf(x.h) < 1e30f ? pair_add(r.base, x) : x;
 }
 

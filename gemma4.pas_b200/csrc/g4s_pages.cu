@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
 {
     cg::cluster_group cluster = cg::this_cluster();
     extern __shared__ int s_dyn[];
-    __shared__ int s_free[PG_WARPS], s_bad, s_over, s_writers[PG_HEADS];
+    __shared__ int s_free[PG_WARPS], s_bad, s_over, s_most, s_writers[PG_HEADS];
     __shared__ int4 s_cta[PG_CLUSTER];  // each CTA's free pages, bad entries, short tables
     __shared__ unsigned long long s_sh[2][PG_WARPS];
     const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
     };
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    if (tid == 0) s_bad = s_over = 0;
+    if (tid == 0) s_bad = s_over = s_most = 0;
     for (int i = tid; i < a.n_in; i += PG_THREADS) s_off[i] = -1;
     s_writers[tid] = -1;
     static_assert(PG_HEADS == PG_THREADS, "one list head a thread");
@@ -106,12 +106,13 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(const __grid_
         s_len[j] = len;
         s_last[j] = last;
     }
-    sync();  // the counts are copied, the children listed
+    for (int i = tid; i < a.n_in; i += PG_THREADS) atomicMax(&s_most, pages_of(max(seq_len(a, i), 0), P));
+    sync();  // the counts are copied, the children listed, the longest old row known
 
     // each old sequence's row goes to its children; its pages lose its hold and gain theirs
-    const int chunks = (a.width + PG_ROW * 32 - 1) / (PG_ROW * 32);
-    for (int task = gw; task < a.n_in * chunks; task += slices) {
-        const int i = task / chunks, c0 = task % chunks * (PG_ROW * 32) + lane;
+    const int chunks = (s_most + PG_ROW * 32 - 1) / (PG_ROW * 32);
+    for (int task = gw; task < a.n_in * chunks; task += slices) {  // (a GPU's memory holds under 2^31 chunks)
+        const int i = task % a.n_in, c0 = task / a.n_in * (PG_ROW * 32) + lane;
         const int n = pages_of(max(seq_len(a, i), 0), P), first = s_off[i];
         if (c0 - lane >= n) continue;
         const int32_t *row = a.tables_in + (int64_t)i * a.width + c0;
@@ -345,12 +346,14 @@ __global__ void __launch_bounds__(PC_THREADS, PC_CTAS) pages_copy_kernel(const _
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if constexpr (!FORK) {
-        for (int i = blockIdx.x; i < a.n_in; i += gridDim.x) {
+        // a CTA an eighth of a sequence's entries, every eighth block of them
+        for (int w = blockIdx.x; w < a.n_in * 8; w += gridDim.x) {
+            const int i = w >> 3;
             const int64_t most = (int64_t)a.width * a.page_tokens;
             const int raw = a.lens_in[i];
             const int len = raw < 0 ? 0 : (int)min((int64_t)raw, most);
-            int bad = threadIdx.x == 0 && len != raw;
-            for (int c = threadIdx.x; c < pages_of(len, a.page_tokens); c += PC_THREADS) {
+            int bad = (w & 7) == 0 && threadIdx.x == 0 && len != raw;
+            for (int c = (w & 7) * PC_THREADS + threadIdx.x; c < pages_of(len, a.page_tokens); c += 8 * PC_THREADS) {
                 const int64_t o = (int64_t)i * a.width + c;
                 int p = a.tables_in[o];
                 if (p >= 0 && p < a.n_pages) {
@@ -439,7 +442,7 @@ template <bool FORK>
 static cudaError_t launch_copy(const PagesArgs &a, const PoolArgs &pools, int sms, cudaStream_t s)
 {
     int64_t work = (int64_t)a.max_copies * pools.n * pools.chunks;
-    if (!FORK && work < a.n_in) work = a.n_in;
+    if (!FORK && work < a.n_in * 8) work = a.n_in * 8;
     if (work == 0) return cudaSuccess;
     const int64_t most = (int64_t)sms * PC_CTAS;
     return launch_dependent(pages_copy_kernel<FORK>, work < most ? work : most, PC_THREADS, 0, s, a, pools);

@@ -142,6 +142,24 @@ int main()
     FORK(out.refs = s.in.refs + 7, G4S_ERR_ARG, "refs or lens")
     FORK(out.lens = s.in.lens + 1, G4S_ERR_ARG, "refs or lens")
     { Fork s; s.n_in = s.n_out = 0; s.in.tables = s.in.lens = s.out.tables = s.out.lens = s.src = nullptr; EXPECT(s.run(), G4S_OK, ""); }
+    // a compaction's and a step's own checks
+    {
+        Fork s;
+        EXPECT(g4s_pages_compact(&C, &s.cache, 2, &s.in, &s.out, ints(40960), ints(45060), s.result, nullptr), G4S_ERR_ARG, "aligned");
+        EXPECT(g4s_pages_compact(&C, &s.cache, 2, &s.in, &s.out, nullptr, ints(45056), s.result, nullptr), G4S_ERR_ARG, "page_map");
+        s.out.tables = s.in.tables + 1;
+        EXPECT(g4s_pages_compact(&C, &s.cache, 2, &s.in, &s.out, ints(40960), ints(45056), s.result, nullptr), G4S_ERR_ARG, "overlap");
+        Select q;
+        q.p.n_out = 5;
+        EXPECT(g4s_beam_step(&C, q.logits, q.dtype, 2, 100, 100, 30.0f, &q.p, &q.in, &q.out, q.parents, q.tokens, nullptr, 0, nullptr, nullptr),
+               G4S_ERR_ARG, "n_out");
+        q.p.n_out = 4;
+        g4s_beam_pages pages{&s.cache, s.in, s.in, 1, s.result};
+        EXPECT(g4s_beam_step(&C, q.logits, q.dtype, 2, 100, 100, 30.0f, &q.p, &q.in, &q.out, q.parents, q.tokens, nullptr, 0, &pages, nullptr),
+               G4S_ERR_ARG, "tables");
+        EXPECT(g4s_beam_step(&C, q.logits, q.dtype, 2, 100, 100, 30.0f, &q.p, &q.in, &q.out, q.parents, q.tokens, nullptr, 1, nullptr, nullptr),
+               G4S_ERR_ARG, "NULL");
+    }
     // entry points without a context
     if (g4s_beam_select(nullptr, nullptr, 0, 1, 1, 1, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr) != G4S_ERR_ARG ||
         g4s_beam_reorder(nullptr, nullptr, 1, 1, nullptr, 0, nullptr) != G4S_ERR_ARG ||

@@ -554,3 +554,18 @@ def test_reorder_rows_over_4_gib_apart(sampler, g4, torch_cuda):
     assert [int(buf[r * row + 63]) for r in range(3)] == [3, 1, 1]
     del buf
     torch.cuda.empty_cache()
+
+
+def test_select_extreme_scores(sampler, g4, torch_cuda):
+    rng = np.random.default_rng(17)
+    x = logits(rng, 12, 3000)
+    scores = np.array([0.0, -1e9, -1e9, -1e9, 5.0, np.inf, -3.0, -2.0, -3e38, -1e30, 1e20, -7.0])
+    c = Case(torch_cuda, g4, x, "f32", 4, 6, scores=scores)
+    s, l, d, p, t = c.run(sampler)
+    want = beam_util.select(c.x, c.scores, c.lens, c.done, 4, 6, 30.0, 1.0, 0.0, 7)
+    # beams held back by a large negative score come in their own order behind the first
+    assert p[0].tolist() == [k[2] for k in want[0][:6]] and t[0].tolist() == [k[3] for k in want[0][:6]]
+    # +inf takes every place, best logits first
+    assert (p[1] == 5).all() and (s[1] == np.inf).all()
+    assert t[1].tolist() == np.lexsort((np.arange(3000), -c.x[5]))[:6].tolist()
+    assert p[2][0] == 10 and np.isfinite(s[2]).all()
