@@ -74,6 +74,7 @@ struct g4s_ctx {
     // LM head workspace (first g4s_lmhead_sample call): fp32 logits and fp16 hidden
     float *lm_logits = nullptr;
     void *lm_xh = nullptr;
+    float4 *beam_stat = nullptr;  // [max_rows][BEAM_MAX_ITEMS] item statistics of g4s_beam_select
     int4 *pg_copies = nullptr;  // [max_rows] page copies a g4s_pages_fork lists, and their count
     int *pg_n_copies = nullptr;
     int *dev_err = nullptr;  // device error flag in the workspace (a bounded wait that ran out), read by g4s_device_status
@@ -516,6 +517,7 @@ int32_t g4s_create(int32_t device, int32_t max_rows, int32_t max_vocab, uint32_t
     const size_t o_tab = off; off = align(off + (size_t)SC_TABLE_BYTES);
     const size_t o_etab = off; off = align(off + (size_t)ETAB_TABLE_BYTES);
     const size_t o_stg = off; off = align(off + (size_t)max_rows * sizeof(ShardTarget));
+    const size_t o_bst = off; off = align(off + (size_t)max_rows * BEAM_MAX_ITEMS * sizeof(float4));
     const size_t o_pgc = off; off = align(off + (size_t)max_rows * sizeof(int4));
     const size_t o_pgn = off; off = align(off + sizeof(int));
     ctx->ws_bytes = off;
@@ -537,6 +539,7 @@ int32_t g4s_create(int32_t device, int32_t max_rows, int32_t max_vocab, uint32_t
     ctx->sc_tab = (float *)(base + o_tab);
     ctx->e_tab = (float *)(base + o_etab);
     ctx->shard_tgt = (ShardTarget *)(base + o_stg);
+    ctx->beam_stat = (float4 *)(base + o_bst);
     ctx->pg_copies = (int4 *)(base + o_pgc);
     ctx->pg_n_copies = (int *)(base + o_pgn);
     if (cudaMemset(ctx->ws, 0, off) != cudaSuccess ||
@@ -1452,7 +1455,7 @@ static int32_t beam_select_args(g4s_ctx *ctx, const char *who, const void *logit
     a.out_done = out->done;
     a.out_parents = out_parents;
     a.out_tokens = out_tokens;
-    a.istat = ctx->istat;
+    a.istat = ctx->beam_stat;
     vec = ((uintptr_t)logits % 16u == 0) && ((row_stride * (int64_t)esize) % 16 == 0);
     return G4S_OK;
 }

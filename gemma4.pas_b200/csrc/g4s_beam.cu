@@ -12,10 +12,11 @@
 // a beam's tokens; the beams' scores meet in pairs of fp32 numbers, for the
 // few tokens that can be among the best.
 //
-// beam_stream_kernel: one pass over the logits.  An item is `upi` 2 KiB units of one
-//   row; a warp reduces it to (m, ref, S): the largest raw logit, a reference in
-//   units of 2 (ref = s(m) k with the softcap, else m), and
-//   S = sum 2^(s_i k - ref) (2^((l_i - ref) k)), k = log2(e) / T.
+// beam_stream_kernel: one pass over the logits.  A row has up to 128 items of one length
+//   (a whole number of 4 KiB loads, or for short rows 1/2 to 1/8 of one); an item is
+//   reduced to (m, ref, S): the largest raw logit, a reference in powers of two (ref =
+//   s(m) k with the softcap, else m), and S = sum 2^(s_i k - ref) (2^((l_i - ref) k)),
+//   k = log2(e) / T.  Items of one load share ref and S, which stands with the largest m.
 // beam_combine_kernel: one CTA a prompt.
 //   1. a warp a beam: the row's sum from its items (as pairs), and its n_out items with the
 //      largest (m, then lowest item);
@@ -264,8 +265,9 @@ __device__ __forceinline__ bool beam_live(const BeamArgs &a, int row)
 //   1  |l| <= cap: the polynomial of 8 coefficients
 //   2  the same with masked logits
 //   3  element by element: |l| > cap, a NaN, a row's ragged end
-// Without softcap way 0 takes all but NaNs and ends: 2^-inf is 0.
-template <int DT, bool VEC, bool CAP>
+// Without softcap way 0 takes all but NaNs and ends: 2^-inf is 0.  PARTS: several items of a
+// load (kept apart: the vectors that live on to the end cost the other kind 3 us of 43).
+template <int DT, bool VEC, bool CAP, bool PARTS>
 __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const __grid_constant__ BeamArgs a)
 {
     using T = DtypeTraits<DT>;
@@ -276,27 +278,27 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
     const int lane = threadIdx.x & 31;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring + (VEC ? (threadIdx.x >> 5) * (BS_STAGES * BS_NV * 32) + lane : 0));
     const int nw = (int)gridDim.x * (BS_THREADS / 32), w0 = (int)blockIdx.x * (BS_THREADS / 32) + (threadIdx.x >> 5);
-    const int step_row = nw / a.ipr, step_item = nw % a.ipr, item_len = a.upi * BeamGeo<DT>::UNIT;
+    const int step_row = nw / a.rpr, step_run = nw % a.rpr;
     struct Load {
-        int row, item, left;  // left: logits from its start to the item's end
+        int row, run, left;  // left: logits from its start to the run's end
         const char *p;
     };
-    auto find = [&](int row, int item) {  // the first live item from here on in the warp's steps
-        for (;; row += step_row, item += step_item) {
-            if (item >= a.ipr) {
-                item -= a.ipr;
+    auto find = [&](int row, int run) {  // the first live run from here on in the warp's steps
+        for (;; row += step_row, run += step_run) {
+            if (run >= a.rpr) {
+                run -= a.rpr;
                 row++;
             }
-            if (row >= a.rows) return Load{row, item, 0, nullptr};
+            if (row >= a.rows) return Load{row, run, 0, nullptr};
             if (beam_live(a, row)) break;
         }
-        const int e0 = item * item_len;
-        return Load{row, item, min(a.vocab - e0, item_len),
+        const int e0 = run * a.run_len;
+        return Load{row, run, min(a.vocab - e0, a.run_len),
                     (const char *)a.logits + ((int64_t)row * a.row_stride + e0) * T::ESIZE + (VEC ? lane * 16 : 0)};
     };
     auto after = [&](const Load &u) {
-        if (u.left > LOAD) return Load{u.row, u.item, u.left - LOAD, u.p + LOAD * T::ESIZE};
-        return u.row < a.rows ? find(u.row + step_row, u.item + step_item) : u;
+        if (u.left > LOAD) return Load{u.row, u.run, u.left - LOAD, u.p + LOAD * T::ESIZE};
+        return u.row < a.rows ? find(u.row + step_row, u.run + step_run) : u;
     };
     auto fetch = [&](const Load &u, uint32_t to) {
         if (VEC && u.left >= LOAD) ring_copy<0>(to, u.p);
@@ -306,9 +308,9 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
 #pragma unroll
     for (int i = 0; i < BEAM_H1; i++) h1[i] = CAP ? two(a.h1[i]) : 0;
     touch_params(a);
-    const int row0 = w0 / a.ipr, item0 = w0 % a.ipr;
+    const int row0 = w0 / a.rpr, run0 = w0 % a.rpr;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    Load cur = find(row0, item0), nx = after(cur);
+    Load cur = find(row0, run0), nx = after(cur);
     float m = NEG_INF, ref = 0.0f;
     uint64_t s0 = 0, s1 = 0;
     uint32_t at = ring;
@@ -385,7 +387,31 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
             float S = x.x + x.y;
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(FULLMASK, S, d);
-            if (lane == 0) a.istat[cur.row * a.ipr + cur.item] = make_float4(m, ref, S, 0.0f);
+            if constexpr (!PARTS) {
+                if (lane == 0) a.istat[cur.row * a.ipr + cur.run] = make_float4(m, ref, S, 0.0f);
+            } else {
+                // lane k: the largest of the load's k-th part, S with the first that is m
+                float mine = NEG_INF;
+#pragma unroll
+                for (int j = 0; j < BS_NV; j++) {
+                    float x = NEG_INF;
+                    if (way < 3) {
+                        float v[T::VW];
+                        T::unpack(r[j], v);
+#pragma unroll
+                        for (int i = 0; i < T::VW; i++) x = fmaxf(x, v[i]);
+                    } else {
+                        for (int i = j * (LOAD / BS_NV) + lane; i < min(n, (j + 1) * (LOAD / BS_NV)); i += 32)
+                            x = fmaxf(x, beam_raw<DT>(T::load1(p, i)));
+                    }
+                    x = warp_max_redux(x);
+                    if (lane == j * a.subs / BS_NV) mine = fmaxf(mine, x);
+                }
+                const unsigned top = __ballot_sync(FULLMASK, lane < a.subs && mine == m);
+                const int item = cur.run * a.subs + lane;
+                if (lane < a.subs && item < a.ipr)
+                    a.istat[cur.row * a.ipr + item] = make_float4(mine, ref, lane == __ffs(top) - 1 ? S : 0.0f, 0.0f);
+            }
             m = NEG_INF;
             ref = 0.0f;
             s0 = s1 = 0;
@@ -620,10 +646,11 @@ __device__ __forceinline__ uint32_t unit_mask(const char *p, int n, int lane, fl
 {
     using T = DtypeTraits<DT>;
     uint32_t m = 0;
-    if (VEC && n >= BeamGeo<DT>::UNIT) {
-        uint4 r[BNV];
+    if (VEC && n % T::VW == 0) {
+        uint4 r[BNV];  // (past the end: NaN)
 #pragma unroll
-        for (int j = 0; j < BNV; j++) r[j] = __ldg((const uint4 *)p + j * 32 + lane);
+        for (int j = 0; j < BNV; j++)
+            r[j] = (j * 32 + lane) * T::VW < n ? __ldg((const uint4 *)p + j * 32 + lane) : make_uint4(~0u, ~0u, ~0u, ~0u);
 #pragma unroll
         for (int j = 0; j < BNV; j++) {
             const uint32_t w[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
@@ -836,18 +863,31 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
         const int o = atomicAdd(&s_m, 1);
         if (o < a.pc) cand[o] = make_ulonglong2(0, beam_tie(w, key, (uint32_t)id));
     };
-    for (int task = warp; task < nsel * a.upi; task += BC_WARPS) {
-        const uint64_t t = first[task / a.upi].y;
-        const int w = tie_beam(t), u = task % a.upi;
+    const int tasks = (a.item_len + UNIT - 1) / UNIT;  // of an item
+    for (int task = warp; task < nsel * tasks; task += BC_WARPS) {
+        const int j = task / tasks, u = (task - j * tasks) * UNIT;
+        const uint64_t t = first[j].y;
+        const int w = tie_beam(t);
         if (s_row[w].kind == BEAM_DONE) {
             if (lane == 0 && u == 0) push(w, 0u, 0);
             continue;
         }
-        const int64_t e0 = ((int64_t)tie_id(t) * a.upi + u) * UNIT;
-        const int n = (int)min((int64_t)UNIT, a.vocab - e0);
+        const int64_t e0 = (int64_t)tie_id(t) * a.item_len + u;
+        const int n = (int)min((int64_t)min(UNIT, a.item_len - u), a.vocab - e0);
         if (n <= 0) continue;
         const char *p = (const char *)a.logits + ((int64_t)(row0 + w) * a.row_stride + e0) * T::ESIZE;
-        for (uint32_t m = unit_mask<DT, VEC>(p, n, lane, beam_floor<DT>(least(w))); m; m &= m - 1) {
+        const uint32_t key0 = least(w);
+        uint32_t m = unit_mask<DT, VEC>(p, n, lane, beam_floor<DT>(key0));
+        if (key0 == BEAM_KEY_MIN && N - j <= 32) {
+            // nothing bounds this beam's tokens: the N - j largest are at or above the
+            // (N - j)-th largest of the lanes' maxima
+            uint32_t k = 0;
+            for (uint32_t q = m; q; q &= q - 1)
+                k = max(k, beam_key<DT>(T::load1(p, mask_place<DT, VEC>(__ffs(q) - 1, lane))));
+            k = __shfl_sync(FULLMASK, warp_sort_desc_u32(k), N - j - 1);
+            if (k) m = unit_mask<DT, VEC>(p, n, lane, beam_floor<DT>(k));
+        }
+        for (; m; m &= m - 1) {
             const int e = mask_place<DT, VEC>(__ffs(m) - 1, lane);
             push(w, beam_key<DT>(T::load1(p, e)), e0 + e);
         }
@@ -866,16 +906,16 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
                 if (lane == 0) push(w, 0u, 0);
                 continue;
             }
-            const int64_t e0 = (int64_t)tie_id(t) * a.upi * UNIT;
-            const int n = (int)min((int64_t)a.upi * UNIT, a.vocab - e0);
+            const int64_t e0 = (int64_t)tie_id(t) * a.item_len;
+            const int n = (int)min((int64_t)a.item_len, a.vocab - e0);
             const char *p = (const char *)a.logits + ((int64_t)(row0 + w) * a.row_stride + e0) * T::ESIZE;
             auto count = [&](uint32_t key, uint32_t but, int upto) {  // of keys key .. but - 1, at places up to `upto`
                 int c = 0;
 #pragma unroll 1
                 for (int u = 0; u < n; u += UNIT) {
                     const char *pu = p + (int64_t)u * T::ESIZE;
-                    uint32_t m = unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(key));
-                    if (but) m &= ~unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(but));
+                    uint32_t m = unit_mask<DT, VEC>(pu, min(n - u, UNIT), lane, beam_floor<DT>(key));
+                    if (but) m &= ~unit_mask<DT, VEC>(pu, min(n - u, UNIT), lane, beam_floor<DT>(but));
                     for (; upto < n && m; m &= m - 1) c += u + mask_place<DT, VEC>(__ffs(m) - 1, lane) <= upto;
                     c += __popc(m);
                 }
@@ -901,7 +941,7 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
             }
             for (int u = 0; u < n; u += UNIT) {
                 const char *pu = p + (int64_t)u * T::ESIZE;
-                for (uint32_t m = unit_mask<DT, VEC>(pu, n - u, lane, beam_floor<DT>(lo)); m; m &= m - 1) {
+                for (uint32_t m = unit_mask<DT, VEC>(pu, min(n - u, UNIT), lane, beam_floor<DT>(lo)); m; m &= m - 1) {
                     const int e = mask_place<DT, VEC>(__ffs(m) - 1, lane);
                     const uint32_t key = beam_key<DT>(T::load1(pu, e));
                     if (key > lo || u + e <= last) push(w, key, e0 + u + e);
@@ -947,31 +987,47 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
     }
 }
 
+template <int DT, bool VEC, bool CAP, bool PARTS>
+static cudaError_t launch_stream(const BeamArgs &a, int sms, cudaStream_t s)
+{
+    static int bps[MAX_DEVICES] = {};
+    const int dev = current_device();
+    if (dev < 0 || dev >= MAX_DEVICES) return cudaErrorInvalidDevice;
+    if (bps[dev] == 0) {
+        const cudaError_t e =
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&bps[dev], beam_stream_kernel<DT, VEC, CAP, PARTS>, BS_THREADS, 0);
+        if (e != cudaSuccess) return e;
+    }
+    const int64_t per = BS_THREADS / 32, most = (int64_t)bps[dev] * sms, blocks = ((int64_t)a.rows * a.rpr + per - 1) / per;
+    return launch_dependent(beam_stream_kernel<DT, VEC, CAP, PARTS>, blocks < most ? blocks : most, BS_THREADS, 0, s, a);
+}
+
 template <int DT, bool VEC, bool CAP>
 static cudaError_t launch_beam_t(BeamArgs &a, int sms, cudaStream_t s)
 {
-    static int bps[MAX_DEVICES] = {};
     static bool ready[MAX_DEVICES] = {};
     const int dev = current_device();
     if (dev < 0 || dev >= MAX_DEVICES) return cudaErrorInvalidDevice;
     cudaError_t e;
     if (!ready[dev]) {
-        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&bps[dev], beam_stream_kernel<DT, VEC, CAP>, BS_THREADS, 0);
-        if (e != cudaSuccess) return e;
         e = cudaFuncSetAttribute(beam_combine_kernel<DT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  BEAM_COMBINE_SMEM_MAX);
         if (e != cudaSuccess) return e;
         ready[dev] = true;
     }
-    const int64_t per = BS_THREADS / 32, most = (int64_t)bps[dev] * sms;
-    // items of two units (one load), longer ones where a row has over BEAM_MAX_ITEMS of them
-    const int unit = BeamGeo<DT>::UNIT, units = (a.vocab + unit - 1) / unit;
-    a.upi = 2 * ((units + 2 * BEAM_MAX_ITEMS - 1) / (2 * BEAM_MAX_ITEMS));
-    a.ipr = (units + a.upi - 1) / a.upi;
-    const int64_t items = (int64_t)a.rows * a.ipr, blocks = (items + per - 1) / per;
-    e = launch_dependent(beam_stream_kernel<DT, VEC, CAP>, blocks < most ? blocks : most, BS_THREADS, 0, s, a);
+    // up to BEAM_MAX_ITEMS items a row: of several loads where there are more, of parts of
+    // one where there are fewer than half (an item has to hold few of the best tokens: 28
+    // bf16 rows of 2520 logits 124 us with whole loads, 17 with parts)
+    const int load = 32 * BS_NV * DtypeTraits<DT>::VW, loads = (a.vocab + load - 1) / load;
+    a.run_len = (loads + BEAM_MAX_ITEMS - 1) / BEAM_MAX_ITEMS * load;
+    a.rpr = (a.vocab + a.run_len - 1) / a.run_len;
+    for (a.subs = BS_NV; a.subs > 1 && loads * a.subs > BEAM_MAX_ITEMS;) a.subs /= 2;
+    a.item_len = a.run_len / a.subs;
+    a.ipr = (a.vocab + a.item_len - 1) / a.item_len;
+    e = a.subs > 1 ? launch_stream<DT, VEC, CAP, true>(a, sms, s) : launch_stream<DT, VEC, CAP, false>(a, sms, s);
     if (e != cudaSuccess) return e;
-    return launch_dependent(beam_combine_kernel<DT, VEC>, a.rows / a.beams, BC_THREADS, (size_t)(2 * a.pe + a.pc + a.n_out) * 16, s, a);
+    return launch_dependent(beam_combine_kernel<DT, VEC>, a.rows / a.beams, BC_THREADS,
+                            (size_t)(2 * a.pe + a.pc + a.n_out) * 16, s, a);
 }
 
 // tanh(q) / q = 1 + q^2 P(q^2) on |q| <= 1/2, P of degree 3 fitted for the least largest

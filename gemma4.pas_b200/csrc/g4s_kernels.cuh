@@ -255,9 +255,11 @@ struct BeamArgs {
     int32_t *out_lens;
     uint8_t *out_done;
     int32_t *out_parents, *out_tokens;
-    float4 *istat;        // [rows][ipr] (m, ref, S, -)
+    float4 *istat;        // [rows][ipr] (m, ref, S, -); room for BEAM_MAX_ITEMS a row
     // set by launch_beam_select
-    int upi, ipr;         // 2 KiB units an item, items a row
+    int item_len, ipr;    // logits of an item, items a row
+    int run_len, rpr;     // logits that a warp of the streaming pass takes at a time, of them a row
+    int subs;             // items of such a run (1, or of one load 2, 4 or 8)
     float k, invcap, lim1, lim2;         // lim1, lim2: largest |logit| of the two polynomials
     float ref32;                         // powers of two a unit of ref
     int skip_min;                        // whether the first polynomial may take any logit below cap / 2
