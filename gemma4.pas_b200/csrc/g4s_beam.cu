@@ -34,6 +34,7 @@ constexpr int BS_THREADS = 128;  // CTA of the streaming pass
 constexpr int BS_CTAS = 6;       // of them on an SM: 80 registers a thread, 32 KiB a CTA
 constexpr int BS_STAGES = 2;     // loads a warp's ring in shared memory holds
 constexpr int BS_NV = 8;         // 16-byte vectors a lane and load (4 KiB, two units)
+constexpr int LINE = 128;        // loads of unaligned rows are copied from the line's start
 constexpr int BC_THREADS = 1024; // CTA of the combine
 constexpr int BC_WARPS = BC_THREADS / 32;
 constexpr int BIPL = BEAM_MAX_ITEMS / 32;  // a row's items a lane of its warp
@@ -74,24 +75,6 @@ __device__ __forceinline__ float beam_soft(float v, const BeamArgs &a)
     const float q = __fmul_rn(v, a.invcap), aq = fabsf(q);
     const float w = 1.0f - __fdividef(2.0f, ex2_approx(aq * (2.0f * G4_L2E)) + 1.0f);
     return __fmul_rn(aq <= 1.0f ? tanh_poly(q) : copysignf(w, q), a.softcap);
-}
-
-// A load of a row that no vector load fits: every 32nd logit (pair of words for bf16).
-template <int DT>
-__device__ __forceinline__ void load_single(const char *p, int lane, uint4 (&r)[BS_NV])
-{
-    uint32_t w[BS_NV * 4];
-#pragma unroll
-    for (int i = 0; i < BS_NV * 4; i++) {
-        if constexpr (DT == G4S_F32) {
-            w[i] = __float_as_uint(__ldg((const float *)p + i * 32 + lane));
-        } else {
-            const unsigned short *h = (const unsigned short *)p + i * 64 + lane;
-            w[i] = (uint32_t)__ldg(h) | ((uint32_t)__ldg(h + 32) << 16);
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < BS_NV; j++) r[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
 }
 
 // Two fp32 numbers in a 64-bit register: the packed operations' operands.  two() is volatile
@@ -245,6 +228,63 @@ __device__ __forceinline__ void ring_read(uint32_t from, uint4 (&r)[BS_NV])
     if constexpr (J + 1 < BS_NV) ring_read<J + 1>(from, r);
 }
 
+// The same of a row that is not 16-byte aligned: its bytes stand `shift` into the ring, and
+// word i of the lane is word i * 32 + lane of the load (two bf16 logits side by side; where
+// they do not share an aligned word, cut from two).
+template <int DT>
+__device__ __forceinline__ void ring_read_shifted(uint32_t from, uint32_t shift, int lane, uint4 (&r)[BS_NV])
+{
+    const uint32_t a = from + (shift & ~3u) + lane * 4;
+    uint32_t w[BS_NV * 4];
+#pragma unroll
+    for (int i = 0; i < BS_NV * 4; i++) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(a + i * 128) : "memory");
+    if (DT == G4S_BF16 && (shift & 2)) {
+#pragma unroll
+        for (int i = 0; i < BS_NV * 4; i++) {
+            uint32_t next;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(next) : "r"(a + i * 128 + 4) : "memory");
+            w[i] = __byte_perm(w[i], next, 0x5432);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < BS_NV; j++) r[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+
+// A load's logits from n on (behind the row's end) become -inf in the ring (in registers the
+// cut costs spills): the lane's own vectors, or, of a load that stands `shift` into the
+// ring, by the whole warp.
+template <int DT>
+__device__ __forceinline__ void ring_low(uint32_t at)  // one logit
+{
+    if constexpr (DT == G4S_BF16) asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"((unsigned short)0xff80) : "memory");
+    else asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(0xff800000u) : "memory");
+}
+template <int DT>
+__device__ __forceinline__ void ring_low16(uint32_t at)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(DT == G4S_BF16 ? 0xff80ff80u : 0xff800000u) : "memory");
+}
+template <int DT>
+__device__ __forceinline__ void ring_cut(uint32_t at, int lane, int n)
+{
+    using T = DtypeTraits<DT>;
+#pragma unroll 1
+    for (int left = n - lane * T::VW, j = 0; j < BS_NV; j++, left -= 32 * T::VW, at += 512) {
+        if (left <= 0) ring_low16<DT>(at);
+        else
+            for (int i = left; i < T::VW; i++) ring_low<DT>(at + i * T::ESIZE);
+    }
+}
+template <int DT>
+__device__ __forceinline__ void ring_cut_shifted(uint32_t from, uint32_t shift, int lane, int n)
+{
+    using T = DtypeTraits<DT>;
+    const uint32_t end = shift + n * T::ESIZE, up = (end + 15) & ~15u;
+    if (lane < (int)(up - end) / T::ESIZE) ring_low<DT>(from + end + lane * T::ESIZE);
+#pragma unroll 1
+    for (uint32_t b = up + lane * 16; b < BS_NV * 512 + LINE; b += 512) ring_low16<DT>(from + b);
+}
+
 // A beam that continues: a score that is not -inf (nor NaN), and not ended.
 __device__ __forceinline__ bool beam_live(const BeamArgs &a, int row)
 {
@@ -254,8 +294,14 @@ __device__ __forceinline__ bool beam_live(const BeamArgs &a, int row)
 }
 
 // Persistent warps over the live rows' items; each lane copies its own vectors of the two
-// loads ahead into the warp's ring (cp.async: no registers, no barrier).  The ways through
-// a load:
+// loads ahead into the warp's ring (cp.async: no registers, no barrier).  Rows that are not
+// 16-byte aligned are copied by the lines that hold them (bytes before the row's first
+// logit in the same line, behind its last in the same 16 bytes) and read from the ring at
+// their offset, so that a row's sums are grouped alike wherever it starts: equal beams
+// score equal.  (256 rows of 262143 logits: bf16 80 -> 50 us, aligned 44; fp32 58 for 57,
+// or 63 where the copies start at 16 bytes.)  A row's ragged end is filled with masked
+// logits in the ring: element by element it took the whole kernel 2 to 10 us longer.  The
+// ways through a load:
 //   0  no logit above cap / 2: the polynomial of 5 coefficients (7 packed operations a
 //      pair).  Below -cap / 2 it falls faster than tanh, to -inf for masked logits (its
 //      last coefficient is positive); with the load's maximum at or above 0 and cap >=
@@ -264,8 +310,8 @@ __device__ __forceinline__ bool beam_live(const BeamArgs &a, int row)
 //      to be at or above -cap / 2
 //   1  |l| <= cap: the polynomial of 8 coefficients
 //   2  the same with masked logits
-//   3  element by element: |l| > cap, a NaN, a row's ragged end
-// Without softcap way 0 takes all but NaNs and ends: 2^-inf is 0.  PARTS: several items of a
+//   3  element by element: |l| > cap, a NaN
+// Without softcap way 0 takes all but NaNs: 2^-inf is 0.  PARTS: several items of a
 // load (kept apart: the vectors that live on to the end cost the other kind 3 us of 43).
 template <int DT, bool VEC, bool CAP, bool PARTS>
 __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const __grid_constant__ BeamArgs a)
@@ -273,10 +319,11 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
     using T = DtypeTraits<DT>;
     constexpr int LOAD = 32 * BS_NV * T::VW;  // logits of a load
     const float NEG_INF = -__uint_as_float(0x7f800000u);
-    __shared__ uint4 s_ring[VEC ? BS_THREADS / 32 * BS_STAGES * BS_NV * 32 : 1];
+    constexpr int STAGE = BS_NV * 512 + (VEC ? 0 : LINE);  // bytes
+    __shared__ uint4 s_ring[BS_THREADS / 32 * BS_STAGES * STAGE / 16];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring + (VEC ? (threadIdx.x >> 5) * (BS_STAGES * BS_NV * 32) + lane : 0));
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring) + (threadIdx.x >> 5) * (BS_STAGES * STAGE) + lane * 16;
     const int nw = (int)gridDim.x * (BS_THREADS / 32), w0 = (int)blockIdx.x * (BS_THREADS / 32) + (threadIdx.x >> 5);
     const int step_row = nw / a.rpr, step_run = nw % a.rpr;
     struct Load {
@@ -301,7 +348,15 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
         return u.row < a.rows ? find(u.row + step_row, u.run + step_run) : u;
     };
     auto fetch = [&](const Load &u, uint32_t to) {
-        if (VEC && u.left >= LOAD) ring_copy<0>(to, u.p);
+        const int shift = VEC ? 0 : (int)((uintptr_t)u.p & (LINE - 1));
+        const char *p = u.p - shift + (VEC ? 0 : lane * 16);
+        if (u.left >= LOAD) {
+            ring_copy<0>(to, p);
+            if (!VEC && lane * 16 < shift) cp_async16s(to + BS_NV * 512, p + BS_NV * 512);
+        } else {
+            const int end = shift + u.left * T::ESIZE;
+            for (int b = lane * 16; b < end; b += 512, p += 512, to += 512) cp_async16s(to, p);
+        }
         cp_async_commit();
     };
     uint64_t h1[BEAM_H1], k2 = two(a.k);
@@ -315,25 +370,28 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
     uint64_t s0 = 0, s1 = 0;
     uint32_t at = ring;
     fetch(cur, ring);
-    fetch(nx, ring + BS_NV * 512);
+    fetch(nx, ring + STAGE);
     while (cur.row < a.rows) {
         uint4 r[BS_NV];
-        const bool whole = cur.left >= LOAD, last = cur.left <= LOAD;
+        const bool last = cur.left <= LOAD;
+        cp_async_wait<1>();
         if constexpr (VEC) {
-            cp_async_wait<1>();
+            if (cur.left < LOAD) ring_cut<DT>(at, lane, cur.left);
             ring_read<0>(at, r);
-        } else if (whole) {
-            load_single<DT>(cur.p, lane, r);
+        } else {
+            const uint32_t from = at - lane * 16, shift = (uint32_t)(uintptr_t)cur.p & (LINE - 1);
+            __syncwarp();  // (the lanes read one another's copies)
+            if (cur.left < LOAD) {
+                ring_cut_shifted<DT>(from, shift, lane, cur.left);
+                __syncwarp();
+            }
+            ring_read_shifted<DT>(from, shift, lane, r);
         }
-        float mx = NEG_INF;
-        int way = 3;
-        if (whole) {
-            mx = lane_max<DT>(r);  // (the loads from the ring are done: it can be refilled)
-            way = __all_sync(FULLMASK, CAP ? mx <= a.lim1 : mx <= beam_max<DT>()) ? 0 : 1;  // a NaN fails
-        }
+        float mx = lane_max<DT>(r);  // (with the vote, every lane's reads of the ring are done: it can be refilled)
+        int way = __all_sync(FULLMASK, CAP ? mx <= a.lim1 : mx <= beam_max<DT>()) ? 0 : 1;  // a NaN fails
         const Load n2 = after(nx);
         fetch(n2, at);
-        if (!whole || (way == 1 && !CAP)) {
+        if (way == 1 && !CAP) {
             way = 3;
         } else if (CAP && (way == 1 || !(a.skip_min && __any_sync(FULLMASK, mx >= 0.0f)))) {
             float mn = lane_min<DT>(r);
@@ -418,7 +476,7 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
         }
         cur = nx;
         nx = n2;
-        at = at == ring ? ring + BS_NV * 512 : ring;
+        at = at == ring ? ring + STAGE : ring;
     }
     cp_async_wait<0>();
 }

@@ -172,10 +172,13 @@ __device__ __forceinline__ void touch_params(const A &a)
 }
 
 // asynchronous copies of 16 bytes into shared memory
+__device__ __forceinline__ void cp_async16s(uint32_t smem, const void *gmem)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
 __device__ __forceinline__ void cp_async16(void *smem, const void *gmem)
 {
-    const uint32_t sa = (uint32_t)__cvta_generic_to_shared(smem);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sa), "l"(gmem) : "memory");
+    cp_async16s((uint32_t)__cvta_generic_to_shared(smem), gmem);
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
