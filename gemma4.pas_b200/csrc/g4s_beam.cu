@@ -37,6 +37,7 @@ constexpr int BS_NV = 8;         // 16-byte vectors a lane and load (4 KiB, two 
 constexpr int LINE = 128;        // loads of unaligned rows are copied from the line's start
 constexpr int BC_THREADS = 1024; // CTA of the combine
 constexpr int BC_WARPS = BC_THREADS / 32;
+constexpr int BEAM_PART_ITEMS = 64;
 constexpr int BIPL = BEAM_MAX_ITEMS / 32;  // a row's items a lane of its warp
 constexpr int BNV = 4;           // 16-byte vectors a lane and unit (2 KiB a unit)
 
@@ -1074,12 +1075,14 @@ static cudaError_t launch_beam_t(BeamArgs &a, int sms, cudaStream_t s)
         ready[dev] = true;
     }
     // up to BEAM_MAX_ITEMS items a row: of several loads where there are more, of parts of
-    // one where there are fewer than half (an item has to hold few of the best tokens: 28
-    // bf16 rows of 2520 logits 124 us with whole loads, 17 with parts)
+    // one where there are few (an item has to hold few of the best tokens: 28 bf16 rows of
+    // 2520 logits 124 us with whole loads, 15 with parts), to BEAM_PART_ITEMS at most (the
+    // parts' maxima cost the streaming pass: 180 bf16 rows of 54 loads 27.2 us in halves,
+    // 24.5 whole; 28 rows of 10 loads 11.5 with 4 parts a load, 12.4 with 2)
     const int load = 32 * BS_NV * DtypeTraits<DT>::VW, loads = (a.vocab + load - 1) / load;
     a.run_len = (loads + BEAM_MAX_ITEMS - 1) / BEAM_MAX_ITEMS * load;
     a.rpr = (a.vocab + a.run_len - 1) / a.run_len;
-    for (a.subs = BS_NV; a.subs > 1 && loads * a.subs > BEAM_MAX_ITEMS;) a.subs /= 2;
+    for (a.subs = BS_NV; a.subs > 1 && loads * a.subs > BEAM_PART_ITEMS;) a.subs /= 2;
     a.item_len = a.run_len / a.subs;
     a.ipr = (a.vocab + a.item_len - 1) / a.item_len;
     e = a.subs > 1 ? launch_stream<DT, VEC, CAP, true>(a, sms, s) : launch_stream<DT, VEC, CAP, false>(a, sms, s);
