@@ -25,6 +25,15 @@
 //      another holds a token that beats all of the other's);
 //   3. these items reread, their tokens above the beam's best item left out
 //      collected (at most n_out - j from the item in place j), ranked, sorted.
+//
+// Measured (one B200, copy bandwidth 6570 GB/s), the whole selection: 256 bf16 rows of
+// 262144 logits, 8 beams, 16 continuations 43 us (3.1 TB/s; the streaming pass 33, without
+// its sums 23); 205 live fp32 rows 47 us (4.6 TB/s; 39, 35); 4 fp32 rows 9.6 us (5.2); 30
+// live fp32 rows of 32003 logits 10.3 us (4.4).  The streaming pass is bound by
+// instructions for bf16 rows (issue slots 58 %, the exponentials' unit 50 %, fp32 pipe
+// 48 % busy at 20 warps an SM) and by memory for fp32; the combine, 4 us for 4 beams and
+// 10 for 8 beams and 16 continuations, by the latency of dependent steps: its one CTA a
+// prompt leaves most of the GPU idle, and waits for barriers and instruction fetches.
 #include "g4s_device.cuh"
 #include "g4s_kernels.cuh"
 
@@ -1137,7 +1146,8 @@ cudaError_t launch_beam_select(BeamArgs &a, int dtype, bool vec, int sms, cudaSt
 // A thread moves one column (sizeof(V) bytes at one place of a segment) of all of a
 // group's rows: every row that is wanted is read before any is written, so that source
 // and destination may be the same memory without a copy or a barrier, and a parent of
-// several rows is read once.
+// several rows is read once.  Bound by memory: 801 MB read and written in 122 us, 6.5 TB/s,
+// the bandwidth of a copy; one prompt's 1.6 MB take 4.3 us, latency.
 template <class V, int WMAX>
 __device__ __forceinline__ void reorder_column(const ReorderTensor &t, int row0, uint32_t c, const uint32_t *child)
 {
