@@ -74,7 +74,7 @@ struct g4s_ctx {
     // LM head workspace (first g4s_lmhead_sample call): fp32 logits and fp16 hidden
     float *lm_logits = nullptr;
     void *lm_xh = nullptr;
-    float4 *beam_stat = nullptr;  // [max_rows][BEAM_MAX_ITEMS] item statistics of g4s_beam_select
+    float4 *beam_stat = nullptr;  // [max_rows][beam_items(max_vocab)] item statistics of g4s_beam_select
     int4 *pg_copies = nullptr;  // [max_rows] page copies a g4s_pages_fork lists, and their count
     int *pg_n_copies = nullptr;
     int *dev_err = nullptr;  // device error flag in the workspace (a bounded wait that ran out), read by g4s_device_status
@@ -517,7 +517,7 @@ int32_t g4s_create(int32_t device, int32_t max_rows, int32_t max_vocab, uint32_t
     const size_t o_tab = off; off = align(off + (size_t)SC_TABLE_BYTES);
     const size_t o_etab = off; off = align(off + (size_t)ETAB_TABLE_BYTES);
     const size_t o_stg = off; off = align(off + (size_t)max_rows * sizeof(ShardTarget));
-    const size_t o_bst = off; off = align(off + (size_t)max_rows * BEAM_MAX_ITEMS * sizeof(float4));
+    const size_t o_bst = off; off = align(off + (size_t)max_rows * beam_items(max_vocab) * sizeof(float4));
     const size_t o_pgc = off; off = align(off + (size_t)max_rows * sizeof(int4));
     const size_t o_pgn = off; off = align(off + sizeof(int));
     ctx->ws_bytes = off;

@@ -237,6 +237,12 @@ inline cudaError_t launch_dependent(void (*kernel)(P...), int64_t blocks, int th
 }
 
 constexpr int BEAM_MAX_ITEMS = 128;  // items a row in the selection's statistics
+// The most items that a row of up to `vocab` logits of either type has: 8 a load of 4 KiB.
+inline int beam_items(int vocab)
+{
+    const int loads = vocab / 1024 + 1;
+    return loads < BEAM_MAX_ITEMS / 8 ? loads * 8 : BEAM_MAX_ITEMS;
+}
 constexpr int BEAM_COMBINE_SMEM_MAX = (2 * 2048 + 4096 + 64) * 16;  // 32 beams, 64 continuations
 constexpr int BEAM_H1 = 5, BEAM_H2 = 8;  // coefficients of the folded softcap polynomials
 
@@ -255,7 +261,7 @@ struct BeamArgs {
     int32_t *out_lens;
     uint8_t *out_done;
     int32_t *out_parents, *out_tokens;
-    float4 *istat;        // [rows][ipr] (m, ref, S, -); room for BEAM_MAX_ITEMS a row
+    float4 *istat;        // [rows][ipr] (m, ref, S, -); room for beam_items a row
     // set by launch_beam_select
     int item_len, ipr;    // logits of an item, items a row
     int run_len, rpr;     // logits that a warp of the streaming pass takes at a time, of them a row

@@ -143,6 +143,44 @@ def test_select_shapes(sampler, g4, torch_cuda, dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("offset", range(8))
+def test_select_row_ends_at_every_alignment(sampler, g4, torch_cuda, dtype, offset):
+    """Rows that end in, at and behind a load, from every place of 16 bytes on; what stands beside them is never seen."""
+    rng = np.random.default_rng(offset)
+    for i, V in enumerate((2, 9, 255, 1023, 1024, 1025, 1031, 2047, 2048, 2049, 4103, 6145)):
+        x = logits(rng, 6, V, 2.5 if i % 3 else 30.0)  # (above the cap too: element by element)
+        c = Case(torch_cuda, g4, x, dtype, 3, 5, pad=(0, 1, 2, 3, 5, 7)[(i + offset) % 6], offset=offset, alpha=0.5,
+                 cap=30.0 if i % 2 else 0.0)
+        rows = c.buf[offset:].view(6, c.stride)
+        for beside in (1e6, np.inf, np.nan):
+            c.buf[:offset] = beside
+            rows[:, V:] = beside
+            c.check(c.run(sampler))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_select_equal_rows_at_any_offset_score_equal(sampler, g4, torch_cuda, dtype):
+    """A row's sums do not depend on where it starts: one prompt's beams of equal logits tie bit for bit."""
+    for V, pad in ((97, 0), (2047, 4), (5003, 2), (40001, 0)):
+        x = np.tile(logits(np.random.default_rng(V), 1, V), (8, 1))
+        c = Case(torch_cuda, g4, x, dtype, 8, 16, pad=pad, scores=np.full(8, -3.0), lens=np.full(8, 2), offset=1)
+        s, _, _, p, t = c.run(sampler)
+        assert p[0].tolist() == list(range(8)) * 2 and len(set(t[0, :8])) == len(set(t[0, 8:])) == 1
+        assert len(set(s[0, :8].tolist())) == len(set(s[0, 8:].tolist())) == 1
+
+
+@pytest.mark.parametrize("max_vocab", [1, 900, 5000, 20000])
+def test_select_in_a_small_context(g4, torch_cuda, max_vocab):
+    """The statistics' room is sized by the context's vocabulary."""
+    s = g4.Sampler(device=0, max_rows=12, max_vocab=max_vocab)
+    rng = np.random.default_rng(max_vocab)
+    for dtype, offset in (("f32", 0), ("f32", 3), ("bf16", 0), ("bf16", 7)):
+        c = Case(torch_cuda, g4, logits(rng, 12, max_vocab), dtype, 4, 6, pad=1, offset=offset)
+        c.check(c.run(s))
+    s.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("cap,T,alpha", [(0.0, 1.0, 0.0), (30.0, 0.5, 0.6), (0.0, 1.7, 1.0), (5.0, 1.0, 2.0),
                                          (1000.0, 0.3, 0.0), (30.0, 1e-3, 0.0), (0.01, 1.0, 0.0)])
 def test_select_parameters(sampler, g4, torch_cuda, dtype, cap, T, alpha):

@@ -172,6 +172,21 @@ def test_fork_large_tables(sampler, g4, torch_cuda):
     run_fork(torch_cuda, g4, sampler, cache, tables, lens, refs, src, 3)
 
 
+def test_fork_more_sequences_than_threads(g4, torch_cuda):
+    s = g4.Sampler(device=0, max_rows=8192, max_vocab=64)
+    rng = np.random.default_rng(6)
+    n, P, width, n_pages = 3000, 3, 5, 30000
+    lens = rng.integers(0, width * P - 1, n)
+    cache = Cache(torch_cuda, g4, rng, n_pages, P, width, layouts=((1, 4, 0, 0),))
+    tables, refs, _ = scattered(rng, n, lens, P, width, n_pages)
+    for n_out in (1025, 8192):
+        src = rng.integers(-1, n, n_out)
+        src[-40:] = src[0]  # a parent whose children are far apart
+        c = Cache(torch_cuda, g4, rng, n_pages, P, width, layouts=((1, 4, 0, 0),))
+        run_fork(torch_cuda, g4, s, c, tables, lens, refs, src, 1, frozen=rng.random(n_out) < 0.2)
+    s.close()
+
+
 def run_compact(torch, g4, sampler, cache, tables, lens, refs, alias):
     cu = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).cuda()
     n, n_pages = len(lens), cache.n_pages
