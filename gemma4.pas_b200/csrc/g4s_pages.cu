@@ -9,8 +9,8 @@
 // steps, so that a fork is two launches whatever its size.  What moves bytes
 // runs over the whole GPU as the first kernel's programmatic dependent.
 //
-// Measured (one B200): fork of one prompt of 4 beams, 1024 pages, 8.2 us (one CTA decides);
-// of 32 prompts of 8 beams, 12288 pages, 13.8 (the cluster); of 8 prompts of 6 beams, up to
+// Measured (one B200): fork of one prompt of 4 beams, 1024 pages, 8.0 us (one CTA decides);
+// of 32 prompts of 8 beams, 12288 pages, 14.0 (the cluster); of 8 prompts of 6 beams, up to
 // 482 pages each, with 5 new positions, 16.3.  Latency bounds them: a few hundred KiB of
 // table entries and counts, about ten dependent steps over them.  Compaction of 8192 pages,
 // 258 MB read and written, 52.5 us: 6 the decision, 46 the copies at 5.6 TB/s (4.9 TB/s in
