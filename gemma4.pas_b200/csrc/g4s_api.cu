@@ -11,6 +11,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <chrono>
 #include <string>
 #include <thread>
@@ -1388,6 +1389,14 @@ static bool aliasing_ok(const void *in, const void *out, size_t in_bytes, size_t
     return a + in_bytes <= b || b + out_bytes <= a;
 }
 
+// Whether all arrays of 4-byte elements stand on their alignment.
+static bool aligned4(std::initializer_list<const void *> arrays)
+{
+    uintptr_t bits = 0;
+    for (const void *p : arrays) bits |= (uintptr_t)p;
+    return bits % 4 == 0;
+}
+
 static int pow2_at_least(int n)
 {
     int p = 4;
@@ -1416,6 +1425,8 @@ static int32_t beam_select_args(g4s_ctx *ctx, const char *who, const void *logit
         return fail(ctx, G4S_ERR_ARG, "%s: row_stride %lld < vocab %d", who, (long long)row_stride, vocab);
     const size_t esize = dtype == G4S_F32 ? 4u : 2u;
     if ((uintptr_t)logits % esize) return fail(ctx, G4S_ERR_ARG, "%s: logits are not aligned to their type", who);
+    if (!aligned4({in->scores, in->lens, out->scores, out->lens, out_parents, out_tokens}))
+        return fail(ctx, G4S_ERR_ARG, "%s: scores, lens, out_parents or out_tokens are not aligned to their type", who);
     if (!(p->temperature >= 1e-6 && p->temperature <= 1e6))
         return fail(ctx, G4S_ERR_ARG, "%s: temperature %g outside [1e-6, 1e6]", who, p->temperature);
     if (!(p->length_alpha >= 0.0 && p->length_alpha <= 8.0))
@@ -1469,6 +1480,7 @@ static int32_t beam_reorder_args(g4s_ctx *ctx, const char *who, const int32_t *p
     if (n_tensors < 0 || n_tensors > G4S_BEAM_MAX_TENSORS)
         return fail(ctx, G4S_ERR_ARG, "%s: n_tensors %d outside [0, %d]", who, n_tensors, G4S_BEAM_MAX_TENSORS);
     if (!parents || (n_tensors && !tensors)) return fail(ctx, G4S_ERR_ARG, "%s: parents or tensors is NULL", who);
+    if (!aligned4({parents})) return fail(ctx, G4S_ERR_ARG, "%s: parents are not aligned to their type", who);
     if (beams < 1 || beams > G4S_BEAM_MAX || groups < 1 || (int64_t)groups * beams > 0x7fffffff - G4S_BEAM_MAX)
         return fail(ctx, G4S_ERR_ARG, "%s: beams %d outside [1, %d], or %d groups", who, beams, G4S_BEAM_MAX, groups);
     a.parents = parents;
@@ -1538,7 +1550,7 @@ static int32_t pages_cache_args(g4s_ctx *ctx, const char *who, const g4s_page_ca
         if (vecs > 0x7fffffff || vecs * c->page_tokens > 0x7fffffff || vecs * c->page_tokens * p.segs > 0x7fffffff)
             return fail(ctx, G4S_ERR_CAPACITY, "%s: pools[%d]: a page of over 2^31 vectors of %d bytes", who, i, q.width);
         const int64_t seg = p.token_bytes * c->page_tokens;
-        if ((p.segs > 1 && p.seg_stride < seg) || p.page_stride < seg + (int64_t)(p.segs - 1) * (p.segs > 1 ? p.seg_stride : 0))
+        if (p.page_stride < seg || (p.segs > 1 && (p.seg_stride < seg || (p.page_stride - seg) / (p.segs - 1) < p.seg_stride)))
             return fail(ctx, G4S_ERR_ARG, "%s: pools[%d]: segments or pages overlap", who, i);
         q.data = (char *)p.data;
         q.page_stride = p.page_stride;
@@ -1570,6 +1582,8 @@ static int32_t pages_fork_args(g4s_ctx *ctx, const char *who, const g4s_page_cac
     if (!in || !out || !result || !in->refs || !out->refs || (n_in && (!in->tables || !in->lens)) ||
         (n_out && (!out->tables || !out->lens || !src)))
         return fail(ctx, G4S_ERR_ARG, "%s: in, out, their arrays, src and result must be non-NULL", who);
+    if (!aligned4({in->tables, in->lens, in->refs, out->tables, out->lens, out->refs, src, result}))
+        return fail(ctx, G4S_ERR_ARG, "%s: tables, lens, refs, src or result are not aligned to their type", who);
     if (n_new < 0 || n_new > 0x3fffffff) return fail(ctx, G4S_ERR_ARG, "%s: n_new %d outside [0, 2^30)", who, n_new);
     const size_t wi = (size_t)n_in * a.width * 4, wo = (size_t)n_out * a.width * 4, np = (size_t)a.n_pages * 4;
     if (n_in && n_out && !aliasing_ok(in->tables, out->tables, wi, wo, false))
@@ -1658,6 +1672,8 @@ int32_t g4s_pages_compact(g4s_ctx *ctx, const g4s_page_cache *cache, int32_t n_s
     if (!in || !out || !page_map || !moves || !result || !in->refs || !out->refs ||
         (n_seqs && (!in->tables || !in->lens || !out->tables)))
         return fail(ctx, G4S_ERR_ARG, "%s: in, out, their arrays, page_map, moves and result must be non-NULL", who);
+    if (!aligned4({in->tables, in->lens, in->refs, out->tables, out->refs, page_map, result}))
+        return fail(ctx, G4S_ERR_ARG, "%s: tables, lens, refs, page_map or result are not aligned to their type", who);
     if ((uintptr_t)moves % 8) return fail(ctx, G4S_ERR_ARG, "%s: moves is not 8-byte aligned", who);
     const size_t w = (size_t)n_seqs * a.width * 4, np = (size_t)a.n_pages * 4;
     if ((n_seqs && !aliasing_ok(in->tables, out->tables, w, w, true)) || !aliasing_ok(in->refs, out->refs, np, np, true))

@@ -74,6 +74,11 @@ int main()
     { Select s; s.vocab = 1001; s.stride = 1001; EXPECT(s.run(), G4S_ERR_CAPACITY, "exceed"); }
     SELECT(stride = 99, G4S_ERR_ARG, "row_stride")
     SELECT(logits = at((1 << 20) + 2), G4S_ERR_ARG, "aligned")
+    SELECT(in.scores = (float *)at(4098), G4S_ERR_ARG, "aligned")
+    SELECT(out.lens = ints(20481), G4S_ERR_ARG, "aligned")
+    SELECT(parents = ints(28674), G4S_ERR_ARG, "aligned")
+    SELECT(tokens = ints(32771), G4S_ERR_ARG, "aligned")
+    SELECT(in.done = (uint8_t *)at(12289), G4S_OK, "")
     SELECT(p.temperature = 0.0, G4S_ERR_ARG, "temperature")
     SELECT(p.temperature = NAN, G4S_ERR_ARG, "temperature")
     SELECT(p.length_alpha = NAN, G4S_ERR_ARG, "length_alpha")
@@ -115,6 +120,7 @@ int main()
     { g4s_beam_tensor t{at(1 << 20), at(1 << 21), 16, 1, 0, 1, 0, 16}; EXPECT(reorder(t, a, blocks, 1, 33), G4S_ERR_ARG, "beams"); }
     { g4s_beam_tensor t{at(1 << 20), at(1 << 21), (int64_t)1 << 34, 1, 0, 1, 0, (int64_t)1 << 33}; EXPECT(reorder(t, a, blocks, 1 << 20, 32), G4S_ERR_CAPACITY, "blocks"); }
     EXPECT(beam_reorder_args(&C, "reorder", ints(4096), 1, 4, nullptr, 33, a, blocks), G4S_ERR_ARG, "n_tensors");
+    EXPECT(beam_reorder_args(&C, "reorder", ints(4098), 1, 4, nullptr, 0, a, blocks), G4S_ERR_ARG, "aligned");
     EXPECT(beam_reorder_args(&C, "reorder", ints(4096), 1, 4, nullptr, 1, a, blocks), G4S_ERR_ARG, "NULL");
 
     EXPECT(Fork().run(), G4S_OK, "");
@@ -130,6 +136,16 @@ int main()
     FORK(pool.token_bytes = 0, G4S_ERR_ARG, "size")
     { Fork s; s.pool.segs = 2; s.pool.seg_stride = 63; s.pool.page_stride = 200; EXPECT(s.run(), G4S_ERR_ARG, "overlap"); }
     { Fork s; s.pool.token_bytes = (int64_t)1 << 36; s.pool.page_stride = (int64_t)1 << 40; EXPECT(s.run(), G4S_ERR_CAPACITY, "vectors"); }
+    // strides whose product is beyond 64 bits
+    { Fork s; s.pool.segs = 3; s.pool.seg_stride = (int64_t)1 << 62; s.pool.page_stride = 4096; EXPECT(s.run(), G4S_ERR_ARG, "overlap"); }
+    { Fork s; s.pool.segs = 5; s.pool.seg_stride = (int64_t)1 << 62; s.pool.page_stride = 4096; EXPECT(s.run(), G4S_ERR_ARG, "overlap"); }
+    { Fork s; s.pool.segs = 3; s.pool.seg_stride = 96; s.pool.page_stride = 256; EXPECT(s.run(), G4S_OK, ""); }
+    { Fork s; s.pool.segs = 3; s.pool.seg_stride = 96; s.pool.page_stride = 255; EXPECT(s.run(), G4S_ERR_ARG, "overlap"); }
+    FORK(in.tables = ints(4097), G4S_ERR_ARG, "aligned")
+    FORK(in.refs = ints(12290), G4S_ERR_ARG, "aligned")
+    FORK(out.lens = ints(20483), G4S_ERR_ARG, "aligned")
+    FORK(src = ints(28673), G4S_ERR_ARG, "aligned")
+    FORK(result = ints(32770), G4S_ERR_ARG, "aligned")
     FORK(n_in = -1, G4S_ERR_ARG, "n_in")
     FORK(n_out = 65, G4S_ERR_CAPACITY, "n_out")
     FORK(n_new = -1, G4S_ERR_ARG, "n_new")
@@ -147,6 +163,7 @@ int main()
         Fork s;
         EXPECT(g4s_pages_compact(&C, &s.cache, 2, &s.in, &s.out, ints(40960), ints(45060), s.result, nullptr), G4S_ERR_ARG, "aligned");
         EXPECT(g4s_pages_compact(&C, &s.cache, 2, &s.in, &s.out, nullptr, ints(45056), s.result, nullptr), G4S_ERR_ARG, "page_map");
+        EXPECT(g4s_pages_compact(&C, &s.cache, 2, &s.in, &s.out, ints(40962), ints(45056), s.result, nullptr), G4S_ERR_ARG, "aligned");
         s.out.tables = s.in.tables + 1;
         EXPECT(g4s_pages_compact(&C, &s.cache, 2, &s.in, &s.out, ints(40960), ints(45056), s.result, nullptr), G4S_ERR_ARG, "overlap");
         Select q;

@@ -404,6 +404,25 @@ def test_reorder(sampler, g4, torch_cuda, in_place, G, W, planes, heads, max_len
     assert np.array_equal(h.cpu().numpy(), hw)
 
 
+def test_reorder_the_most_tensors(sampler, g4, torch_cuda):
+    torch = torch_cuda
+    rng = np.random.default_rng(8)
+    G, W = 3, 4
+    parents = (np.arange(G * W) // W * W + rng.integers(0, W, G * W)).astype(np.int32)
+    host, dev, tens = [], [], []
+    for i in range(g4.BEAM_MAX_TENSORS):
+        n = (1, 4, 16, 5, 4096, 1028, 333)[i % 7]  # bytes a row, every width
+        host.append(rng.integers(0, 256, (G * W, n), dtype=np.uint8))
+        dev.append(torch.from_numpy(host[-1].copy()).cuda())
+        tens.append(g4.BeamTensor(dev[-1].data_ptr(), dev[-1].data_ptr(), n, 1, 0, 1, 0, n))
+    d = torch.from_numpy(parents).cuda()
+    torch.cuda.synchronize()
+    sampler.beam_reorder(d.data_ptr(), G, W, g4.beam_tensors(tens))
+    torch.cuda.synchronize()
+    for h, v in zip(host, dev):
+        assert np.array_equal(v.cpu().numpy(), h[parents])
+
+
 def test_reorder_ignores_parents_of_other_groups(sampler, g4, torch_cuda):
     torch = torch_cuda
     x = torch.arange(8 * 4, dtype=torch.int32, device="cuda").view(8, 4)

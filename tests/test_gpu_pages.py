@@ -466,6 +466,18 @@ def test_tables_without_pools(sampler, g4, torch_cuda):
     run_fork(torch_cuda, g4, sampler, cache, np.full((0, 20), -1), [], refs, [-1, -1], 3)
 
 
+def test_the_most_pools(sampler, g4, torch_cuda):
+    rng = np.random.default_rng(9)
+    layouts = tuple((1 + i % 3, (4, 16, 1, 20)[i % 4], i % 5, i % 2) for i in range(g4.PAGES_MAX_POOLS))
+    P, width, n_pages = 4, 6, 60
+    lens = rng.integers(1, width * P - 2, 6)
+    cache = Cache(torch_cuda, g4, rng, n_pages, P, width, layouts=layouts)
+    tables, refs, _ = scattered(rng, 6, lens, P, width, n_pages)
+    run_fork(torch_cuda, g4, sampler, cache, tables, lens, refs, [0, 0, 1, 3, 3, 3], 1)
+    cache = Cache(torch_cuda, g4, rng, n_pages, P, width, layouts=layouts)
+    assert run_compact(torch_cuda, g4, sampler, cache, tables, lens, refs, False)[1] > 0
+
+
 def test_pages_over_4_gib_in(g4, sampler, torch_cuda):
     torch = torch_cuda
     P, token, n_pages = 4, 1 << 18, 5000  # pages of 1 MiB
