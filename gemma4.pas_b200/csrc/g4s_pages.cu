@@ -13,7 +13,7 @@
 // of 32 prompts of 8 beams, 12288 pages, 14.0 (the cluster); of 8 prompts of 6 beams, up to
 // 482 pages each, with 5 new positions, 16.3.  Latency bounds them: a few hundred KiB of
 // table entries and counts, about ten dependent steps over them.  Compaction of 8192 pages,
-// 258 MB read and written, 52.5 us: 6 the decision, 46 the copies at 5.6 TB/s (4.9 TB/s in
+// 258 MB read and written, 48.3 us: 6 the decision, 42 the copies at 6.1 TB/s (5.3 TB/s in
 // all, of 6.6 for a plain copy).
 #include <cooperative_groups.h>
 
@@ -455,7 +455,11 @@ static cudaError_t launch_copy(const PagesArgs &a, const PoolArgs &pools, int sm
     int64_t work = (int64_t)a.max_copies * pools.n * pools.chunks;
     if (!FORK && work < a.n_in * 8) work = a.n_in * 8;
     if (work == 0) return cudaSuccess;
-    const int64_t most = (int64_t)sms * PC_CTAS;
+    // a compaction's CTAs: as many as fit at once, or four times that where each of these would
+    // have 6 pieces or more, so that they end together (2048 pieces 10.6 us for 11.5, 3072
+    // either way 11.5, 4096 18.6 for 19.0, 16384 48.3 for 52.6; one piece a CTA 61.7).  A
+    // fork's copies are few.
+    const int64_t fit = (int64_t)sms * PC_CTAS, most = FORK || work < 6 * fit ? fit : 4 * fit;
     return launch_dependent(pages_copy_kernel<FORK>, work < most ? work : most, PC_THREADS, 0, s, a, pools);
 }
 
