@@ -39,8 +39,8 @@
 
 namespace g4s {
 
-constexpr int BS_THREADS = 128;  // CTA of the streaming pass
-constexpr int BS_CTAS = 6;       // of them on an SM: 80 registers a thread, 32 KiB a CTA
+constexpr int BS_THREADS = 32;   // CTA of the streaming pass: a warp, which shares nothing with another
+constexpr int BS_CTAS = 24;      // of them on an SM: 80 registers a thread, 8 KiB a CTA
 constexpr int BS_STAGES = 2;     // loads a warp's ring in shared memory holds
 constexpr int BS_NV = 8;         // 16-byte vectors a lane and load (4 KiB, two units)
 constexpr int LINE = 128;        // loads of unaligned rows are copied from the line's start
@@ -303,7 +303,7 @@ __device__ __forceinline__ bool beam_live(const BeamArgs &a, int row)
     return score > -__uint_as_float(0x7f800000u) && !done;
 }
 
-// Persistent warps over the live rows' items; each lane copies its own vectors of the two
+// Long-lived warps over the live rows' items; each lane copies its own vectors of the two
 // loads ahead into the warp's ring (cp.async: no registers, no barrier).  Rows that are not
 // 16-byte aligned are copied by the lines that hold them (bytes before the row's first
 // logit in the same line, behind its last in the same 16 bytes) and read from the ring at
@@ -1090,7 +1090,16 @@ static cudaError_t launch_stream(const BeamArgs &a, int sms, cudaStream_t s)
             cudaOccupancyMaxActiveBlocksPerMultiprocessor(&bps[dev], beam_stream_kernel<DT, VEC, CAP, PARTS>, BS_THREADS, 0);
         if (e != cudaSuccess) return e;
     }
-    const int64_t per = BS_THREADS / 32, most = (int64_t)bps[dev] * sms, blocks = ((int64_t)a.rows * a.rpr + per - 1) / per;
+    // as many times the CTAs that fit as leave four loads each, so that they end together: 256
+    // bf16 rows of 128 loads 42.5 us with 1, 41.6 with 2, 42.5 with 3, 42.2 with 4; 205 live
+    // fp32 rows of 256 loads 47.0, 45.7, 45.0, 44.1; but 248 fp32 rows of 30 loads 16.4 with
+    // 1, 18.2 with 4.  (CTAs of four warps: 4 rows 9.7 us for 9.15, 30 rows of 32003 logits
+    // 10.2 for 9.8.)
+    static_assert(BS_THREADS == 32, "a CTA takes one run at a time");
+    const int64_t blocks = (int64_t)a.rows * a.rpr, fit = (int64_t)bps[dev] * sms;
+    const int64_t loads = blocks * (a.run_len / (32 * BS_NV * DtypeTraits<DT>::VW));
+    int64_t most = fit;
+    for (int m = 2; m <= 4 && loads >= 4 * fit * m; m++) most = fit * m;
     return launch_dependent(beam_stream_kernel<DT, VEC, CAP, PARTS>, blocks < most ? blocks : most, BS_THREADS, 0, s, a);
 }
 
