@@ -28,10 +28,10 @@
 //
 // Measured (one B200, copy bandwidth 6570 GB/s), the whole selection: 256 bf16 rows of
 // 262144 logits, 8 beams, 16 continuations 42 us (3.2 TB/s; the streaming pass 32, without
-// its sums 23); 205 live fp32 rows 47 us (4.6 TB/s; 39, 35); 4 fp32 rows 9.6 us (5.2); 30
-// live fp32 rows of 32003 logits 10.3 us (4.4).  The streaming pass is bound by
-// instructions for bf16 rows (issue slots 60 %, the exponentials' unit 51 %, fp32 pipe
-// 49 % busy at 20 warps an SM) and by memory for fp32; the combine, 4 us for 4 beams and
+// its sums 23); 205 live fp32 rows 44 us (4.9 TB/s; 37, 35); 4 fp32 rows 9.2 us (5.0); 30
+// live fp32 rows of 32003 logits 9.9 us (4.2).  The streaming pass is bound by
+// instructions for bf16 rows (issue slots 58 %, the exponentials' unit 51 %, fp32 pipe
+// 48 % busy at 21 warps an SM) and by memory for fp32; the combine, 4 us for 4 beams and
 // 10 for 8 beams and 16 continuations, by the latency of dependent steps: its one CTA a
 // prompt leaves most of the GPU idle, and waits for barriers and instruction fetches.
 #include "g4s_device.cuh"
@@ -308,7 +308,7 @@ __device__ __forceinline__ bool beam_live(const BeamArgs &a, int row)
 // 16-byte aligned are copied by the lines that hold them (bytes before the row's first
 // logit in the same line, behind its last in the same 16 bytes) and read from the ring at
 // their offset, so that a row's sums are grouped alike wherever it starts: equal beams
-// score equal.  (256 rows of 262143 logits: bf16 48 us, aligned 42; fp32 58 for 56, or 63
+// score equal.  (256 rows of 262143 logits: bf16 46 us, aligned 42; fp32 56 for 54, or 5 more
 // where the copies start at 16 bytes.)  A row's ragged end is filled with masked
 // logits in the ring: element by element it took the whole kernel 2 to 10 us longer.  The
 // ways through a load:
