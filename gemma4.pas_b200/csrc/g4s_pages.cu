@@ -456,9 +456,9 @@ static cudaError_t launch_copy(const PagesArgs &a, const PoolArgs &pools, int sm
     if (!FORK && work < a.n_in * 8) work = a.n_in * 8;
     if (work == 0) return cudaSuccess;
     // a compaction's CTAs: as many as fit at once, or four times that where each of these would
-    // have 6 pieces or more, so that they end together (2048 pieces 10.6 us for 11.5, 3072
-    // either way 11.5, 4096 18.6 for 19.0, 16384 48.3 for 52.6; one piece a CTA 61.7).  A
-    // fork's copies are few.
+    // have 6 pieces or more, so that they end together (one and four times: 2048 pieces 10.6
+    // and 11.5 us, 4096 19.0 and 18.6, 16384 52.6 and 48.3; a CTA a piece 61.7).  A fork's
+    // copies are few.
     const int64_t fit = (int64_t)sms * PC_CTAS, most = FORK || work < 6 * fit ? fit : 4 * fit;
     return launch_dependent(pages_copy_kernel<FORK>, work < most ? work : most, PC_THREADS, 0, s, a, pools);
 }
