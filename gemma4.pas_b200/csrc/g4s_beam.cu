@@ -546,9 +546,13 @@ __device__ __forceinline__ Pair pair_mul(Pair a, Pair b)
     return pair_norm(p, __fmaf_rn(a.h, b.l, __fmaf_rn(a.l, b.h, __fmaf_rn(a.h, b.h, -p))));
 }
 
-// e^z for -80 <= z <= 80: z = n ln2 / 4 + f, |f| <= ln2 / 8, the Taylor series to f^6 (its
-// first terms as pairs), times 2^(n / 4).
-static __device__ __noinline__ Pair pair_exp(Pair z)
+// e^z for -180 <= z <= 80, as v 2^e with 1/2 < v < 2: z = n ln2 / 4 + f, |f| <= ln2 / 8, the
+// Taylor series to f^6 (its first terms as pairs), times 2^(n / 4).
+struct Scaled {
+    Pair v;
+    int e;
+};
+static __device__ __noinline__ Scaled pair_exp_scaled(Pair z)
 {
     const float t = rintf(__fmul_rn(z.h, 5.770780087f));
     const int n = (int)t;
@@ -566,9 +570,13 @@ static __device__ __noinline__ Pair pair_exp(Pair z)
     const int q = n & 3;
     const Pair root = q < 2 ? (q ? Pair{1.189207077f, 3.797635273e-08f} : Pair{1.0f, 0.0f})
                             : (q == 2 ? Pair{1.414213538f, 2.420323497e-08f} : Pair{1.681792855f, -2.475532668e-08f});
-    const Pair v = pair_mul(e, root);
-    const float scale = pow2i(n >> 2);
-    return {v.h * scale, v.l * scale};
+    return {pair_mul(e, root), n >> 2};
+}
+__device__ __forceinline__ Pair pair_exp(Pair z)  // |z| <= 80
+{
+    const Scaled x = pair_exp_scaled(z);
+    const float scale = pow2i(x.e);
+    return {x.v.h * scale, x.v.l * scale};
 }
 
 // log s for 2^-60 <= s <= 2^60: a first value by the hardware, then ln(s e^-y) from its
@@ -585,10 +593,16 @@ __device__ __forceinline__ Pair pair_log(Pair s)
 
 enum { BEAM_DEAD = 0, BEAM_LIVE = 1, BEAM_DONE = 2 };
 struct BeamRow {
-    Pair base, inv;  // score less log of the row's sum (with the softcap less ref too); 1 / max(length, 1)^alpha
+    Pair base;   // score less log of the row's sum (with the softcap less ref too)
+    Scaled inv;  // 1 / max(length, 1)^alpha (to 2^-248: alpha 8, 2^31 tokens)
     float score, ref;
     int len, kind;
 };
+__device__ __forceinline__ Scaled beam_length_power(int length, Pair alpha)
+{
+    const Pair ln = pair_log(pair_sum((float)(length & 0xffff), (float)(length & 0x7fff0000)));
+    return pair_exp_scaled(pair_mul(ln, Pair{-alpha.h, -alpha.l}));
+}
 
 // What a logit adds to its row's base: cap tanh(l / cap) / T, tanh(q) = 1 - 2 / (e^2q + 1)
 // (its cancellation for small q costs 3e-11 of the cap), or (l - ref) / T.
@@ -621,11 +635,23 @@ __device__ __forceinline__ Pair beam_score(const BeamRow &r, Pair x)
     return fabsf(x.h) < 1e30f ? pair_add(r.base, x) : x;
 }
 
-// A pair as a whole number that orders as it does, and its bits.
+// A pair as a whole number that orders as it does, and its bits.  With a length power,
+// whose exponent may leave fp32's range: sign, 10 bits of exponent, h's mantissa, and l in
+// 2^-30 of h's last place.
 __device__ __forceinline__ uint64_t beam_rank(const BeamRow &r, Pair score, bool scaled)
 {
-    if (scaled && fabsf(score.h) < 1e30f) score = pair_mul(score, r.inv);
-    return ((uint64_t)f2key(score.h + 0.0f) << 32) | f2key(score.l + 0.0f);
+    if (!scaled) return ((uint64_t)f2key(score.h + 0.0f) << 32) | f2key(score.l + 0.0f);
+    int e = 0;
+    if (fabsf(score.h) < 1e30f) {
+        score = pair_mul(score, r.inv.v);
+        e = r.inv.e;
+    }
+    const uint32_t b = __float_as_uint(fabsf(score.h));
+    const int eh = (int)(b >> 23);
+    const float l = (score.h < 0.0f ? -score.l : score.l) * pow2i(127 - min(eh, 253));  // |l| <= 2^-24
+    uint64_t m = ((uint64_t)(eh + e + 512) << 53 | (uint64_t)(b & 0x7fffffu) << 30) + (int64_t)rintf(l * 0x1p53f);
+    if (b == 0) m = 0;
+    return score.h < 0.0f ? ~(m | 1ull << 63) : m | 1ull << 63;
 }
 __device__ __forceinline__ uint64_t pair_bits(Pair x) { return ((uint64_t)__float_as_uint(x.h) << 32) | __float_as_uint(x.l); }
 __device__ __forceinline__ Pair bits_pair(uint64_t b) { return {__uint_as_float((uint32_t)(b >> 32)), __uint_as_float((uint32_t)b)}; }
@@ -826,7 +852,7 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
         const uint32_t best = __reduce_max_sync(FULLMASK, kmax);
         const bool live = kind == BEAM_LIVE && best;
         if (sums) {
-            BeamRow r{{0.0f, 0.0f}, {1.0f, 0.0f}, score, 0.0f, len, kind};
+            BeamRow r{{0.0f, 0.0f}, {{1.0f, 0.0f}, 0}, score, 0.0f, len, kind};
             if (live) {
                 float ref = NEG_INF;
 #pragma unroll
@@ -849,11 +875,8 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
                 if (a.softcap > 0.0f)  // ref is in powers of two
                     r.base = pair_add(r.base, pair_mul(Pair{-r.ref, 0.0f}, Pair{0.693147182f, -1.904654212e-09f}));
             }
-            if (a.alpha2[0] != 0.0f) {
-                const int length = max(kind == BEAM_LIVE ? len + 1 : len, 1);
-                const Pair ln = pair_log(pair_sum((float)(length & 0xffff), (float)(length & 0x7fff0000)));
-                r.inv = pair_exp(pair_mul(ln, Pair{-a.alpha2[0], -a.alpha2[1]}));
-            }
+            if (a.alpha2[0] != 0.0f)
+                r.inv = beam_length_power(max(kind == BEAM_LIVE ? len + 1 : len, 1), Pair{a.alpha2[0], a.alpha2[1]});
             if (lane == 0) s_row[w] = r;
             __syncwarp();
             if (pairs) asm volatile("bar.arrive %0, 64;" ::"r"(1 + w) : "memory");
