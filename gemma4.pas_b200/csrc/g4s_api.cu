@@ -1433,6 +1433,8 @@ static int32_t beam_select_args(g4s_ctx *ctx, const char *who, const void *logit
         return fail(ctx, G4S_ERR_ARG, "%s: length_alpha %g outside [0, 8]", who, p->length_alpha);
     if (!(softcap <= 0.0f || (softcap >= 1e-6f && softcap <= 1e6f)))
         return fail(ctx, G4S_ERR_ARG, "%s: softcap %g is neither <= 0 nor within [1e-6, 1e6]", who, softcap);
+    if (softcap > 1e8 * p->temperature)
+        return fail(ctx, G4S_ERR_ARG, "%s: softcap %g is over 1e8 times temperature %g", who, softcap, p->temperature);
     if (p->n_eos < 0 || p->n_eos > G4S_BEAM_MAX_EOS)
         return fail(ctx, G4S_ERR_ARG, "%s: n_eos %d outside [0, %d]", who, p->n_eos, G4S_BEAM_MAX_EOS);
     if (!in->lens && (p->length_alpha != 0.0 || out->lens))

@@ -17,6 +17,8 @@
 //   reduced to (m, ref, S): the largest raw logit, a reference in powers of two (ref =
 //   s(m) k with the softcap, else m), and S = sum 2^(s_i k - ref) (2^((l_i - ref) k)),
 //   k = log2(e) / T.  Items of one load share ref and S, which stands with the largest m.
+//   ref is a rounded number: what it is off by is in every term alike, and the combine
+//   takes it out again, so that a score is base + x(l) - x(row's largest) with both x exact.
 // beam_combine_kernel: one CTA a prompt.
 //   1. a warp a beam: the row's sum from its items (as pairs), and its n_out items with the
 //      largest (m, then lowest item);
@@ -78,13 +80,82 @@ __device__ __forceinline__ uint32_t beam_key(float v)
 // cap * tanh(v / cap) in fp32: the polynomial up to |q| = 1, 1 - 2 / (e^2q + 1) beyond
 // (2 / (e^2q + 1) < 0.24 there, so the approximate exponential and quotient cost less
 // than half an ulp of the result).
-template <bool CAP>
 __device__ __forceinline__ float beam_soft(float v, const BeamArgs &a)
 {
-    if (!CAP) return v;
     const float q = __fmul_rn(v, a.invcap), aq = fabsf(q);
     const float w = 1.0f - __fdividef(2.0f, ex2_approx(aq * (2.0f * G4_L2E)) + 1.0f);
     return __fmul_rn(aq <= 1.0f ? tanh_poly(q) : copysignf(w, q), a.softcap);
+}
+
+// The softcap's kinds.  CAP_FOLD, cap / T up to BEAM_FOLD: s(l) k to a few fp32 steps, so that a
+// term is off by up to 4 * 2^-24 cap / T of itself.  CAP_FAR, beyond: what a term is off by goes
+// with its distance from the maximum and not with the size of the numbers.
+enum { CAP_NONE = 0, CAP_FOLD = 1, CAP_FAR = 2 };
+
+// s(m) k - minus by the very operations that a term takes: with it for a reference and for
+// what the maximum's own term is off by, an error common to the terms falls out.
+template <int CAP>
+__device__ __forceinline__ float beam_value(const BeamArgs &a, float m, float minus)
+{
+    const float q = __fmul_rn(m, m);
+    if constexpr (CAP == CAP_FAR) {
+        float p = a.h1[BEAM_H1 - 1];
+#pragma unroll
+        for (int i = BEAM_H1 - 2; i > 0; i--) p = __fmaf_rn(p, q, a.h1[i]);
+        return __fmaf_rn(__fmul_rn(m, q), p, __fmaf_rn(m, a.h1[0], -minus));
+    }
+    if (fabsf(m) <= a.lim1) {
+        float p = a.h1[BEAM_H1 - 1];
+#pragma unroll
+        for (int i = BEAM_H1 - 2; i >= 0; i--) p = __fmaf_rn(p, q, a.h1[i]);
+        return __fmaf_rn(m, p, -minus);
+    }
+    if (fabsf(m) <= a.lim2) {
+        float p = a.h2[BEAM_H2 - 1];
+#pragma unroll
+        for (int i = BEAM_H2 - 2; i >= 0; i--) p = __fmaf_rn(p, q, a.h2[i]);
+        return __fmaf_rn(m, p, -minus);
+    }
+    return __fmaf_rn(beam_soft(m, a), a.k, -minus);
+}
+
+// CAP_FAR: sums whose maximum the polynomial reaches stand against its value there, rounded
+// (ref), the others against s(m) k itself; the former's own maximum is 2^this.
+__device__ __forceinline__ float beam_off(const BeamArgs &a, float m, float ref)
+{
+    return fabsf(m) <= a.lim1 ? beam_value<CAP_FAR>(a, m, ref) : 0.0f;
+}
+
+// (s(m) - s(l)) k for m >= l to some 2^-21 of itself, whatever cap, T, m and l: with
+// a = m / cap, b = l / cap
+//   tanh a - tanh b = sinh(a - b) / (cosh a cosh b)
+//                   = 2 F (1 - e^-2(a - b)) / ((1 + e^-2|a|) (1 + e^-2|b|)),
+// F = e^-2 min(|a|, |b|) where a and b are on one side of 0, else 1.
+__device__ __forceinline__ float beam_e2(const BeamArgs &a, float v)  // e^-2|v / cap|
+{
+    const float x = fminf(fabsf(v), a.sat), h = __fmul_rn(x, a.two2[0]);
+    const float l = __fmaf_rn(x, a.two2[1], __fmaf_rn(x, a.two2[0], -h));
+    const float e = ex2_approx(-h);
+    return __fmaf_rn(e, -l * 0.693147182f, e);
+}
+__device__ __forceinline__ float beam_below(const BeamArgs &a, float m, float l)
+{
+    const float em = beam_e2(a, m), el = beam_e2(a, l), d = __fmul_rn(__fsub_rn(m, l), a.invcap);
+    const float t = tanh_poly(fminf(d, 1.0f));
+    float num = d <= 1.0f ? 2.0f * t : 1.0f - ex2_approx(d * (-2.0f * G4_L2E));
+    float den = d <= 1.0f ? 1.0f + t : 1.0f;
+    num *= l >= 0.0f ? el : m <= 0.0f ? em : 1.0f;
+    den *= (1.0f + em) * (1.0f + el);
+    return __fmul_rn(a.capk2, __fdividef(num, den));
+}
+// A logit below which (s(m) - s(l)) k is over 64 (set for 96; a term is under 2^-64 of the
+// maximum's, all of a row's together under 2^-41 of its sum): tanh a - tanh b = 192 / (2 cap k).
+__device__ __forceinline__ float beam_nothing(const BeamArgs &a, float m)
+{
+    const float em = beam_e2(a, m), u = (m >= 0.0f ? 2.0f * em : 2.0f) / (1.0f + em) + 192.0f / a.capk2;
+    float lg;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"((2.0f - u) / u));
+    return u < 2.0f ? 0.346573591f * a.softcap * lg : -__uint_as_float(0x7f800000u);
 }
 
 // Two fp32 numbers in a 64-bit register: the packed operations' operands.  two() is volatile
@@ -185,8 +256,9 @@ __device__ __forceinline__ void lane_extremes_open(const uint4 (&r)[BS_NV], floa
 // Adds 2^(s_i k - ref) (without softcap 2^((l_i - ref) k): the difference first, so that
 // k's rounding acts on the distance only) of a load to the lane's sums.  With the softcap
 // s k = l H(l^2), H a polynomial of NH coefficients with k and the cap folded in.  MASKED:
-// some logits add nothing.
-template <int DT, int NH, bool MASKED>
+// some logits add nothing.  APART: the linear part against ref by itself, so that only the
+// rest (under a thirteenth of s k below cap / 2) is rounded before its difference is taken.
+template <int DT, int NH, bool MASKED, bool APART = false>
 __device__ __forceinline__ void load_sum(const uint4 (&r)[BS_NV], const uint64_t *h, uint64_t k, float ref, uint64_t &s0, uint64_t &s1)
 {
     using T = DtypeTraits<DT>;
@@ -203,8 +275,8 @@ __device__ __forceinline__ void load_sum(const uint4 (&r)[BS_NV], const uint64_t
                 const uint64_t q = mul2(v, v);
                 uint64_t p = h[NH - 1];
 #pragma unroll
-                for (int c = NH - 2; c >= 0; c--) p = fma2(p, q, h[c]);
-                y = fma2(v, p, nref);
+                for (int c = NH - 2; c >= (APART ? 1 : 0); c--) p = fma2(p, q, h[c]);
+                y = APART ? fma2(mul2(v, q), p, fma2(v, h[0], nref)) : fma2(v, p, nref);
             } else {
                 y = mul2(add2(v, nref), k);
             }
@@ -321,9 +393,11 @@ __device__ __forceinline__ bool beam_live(const BeamArgs &a, int row)
 //   1  |l| <= cap: the polynomial of 8 coefficients
 //   2  the same with masked logits
 //   3  element by element: |l| > cap, a NaN
+// CAP_FAR has 0 (up to 512 T, its linear part apart) and 3, by differences; vectors without
+// a term (beam_nothing) are passed over there.
 // Without softcap way 0 takes all but NaNs: 2^-inf is 0.  PARTS: several items of a
 // load (kept apart: the vectors that live on to the end cost the other kind 3 us of 43).
-template <int DT, bool VEC, bool CAP, bool PARTS>
+template <int DT, bool VEC, int CAP, bool PARTS>
 __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const __grid_constant__ BeamArgs a)
 {
     using T = DtypeTraits<DT>;
@@ -406,24 +480,26 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
             old_at = -1;
         }
         float mx = lane_max<DT>(r);  // (with the vote, every lane's reads of the ring are done: it can be refilled)
-        int way = __all_sync(FULLMASK, CAP ? mx <= a.lim1 : mx <= beam_max<DT>()) ? 0 : 1;  // a NaN fails
+        int way = __all_sync(FULLMASK, CAP != CAP_NONE ? mx <= a.lim1 : mx <= beam_max<DT>()) ? 0 : 1;  // a NaN fails
         const Load n2 = after(nx);
         fetch(n2, at);
-        if (way == 1 && !CAP) {
+        if (way == 1 && CAP == CAP_NONE) {
             way = 3;
-        } else if (CAP && (way == 1 || !(a.skip_min && __any_sync(FULLMASK, mx >= 0.0f)))) {
+        } else if (CAP != CAP_NONE && (way == 1 || !(a.skip_min && __any_sync(FULLMASK, mx >= 0.0f)))) {
             float mn = lane_min<DT>(r);
             if (way == 1 || !__all_sync(FULLMASK, mn >= -a.lim1)) {
-                way = __all_sync(FULLMASK, mx <= a.lim2 && mn >= -a.lim2) ? 1 : 3;
+                way = CAP == CAP_FOLD && __all_sync(FULLMASK, mx <= a.lim2 && mn >= -a.lim2) ? 1 : 3;
                 if (way == 3) {
                     lane_extremes_open<DT>(r, mx, mn);
-                    if (__all_sync(FULLMASK, mx <= a.lim2 && mn >= -a.lim2)) way = 2;
+                    if (CAP == CAP_FOLD && __all_sync(FULLMASK, mx <= a.lim2 && mn >= -a.lim2)) way = 2;
+                    mx = fminf(mx, beam_max<DT>());
                 }
             }
         }
+        if (CAP == CAP_FAR && m > a.lim1) way = 3;  // the item's sum stands against a maximum beyond the polynomial
         const char *p = cur.p - (VEC ? lane * 16 : 0);
         const int n = min(cur.left, LOAD);
-        if (way == 3) {
+        if (way == 3 && CAP == CAP_NONE) {
             mx = NEG_INF;
 #pragma unroll 4
             for (int i = lane; i < n; i += 32) mx = fmaxf(mx, beam_raw<DT>(T::load1(p, i)));
@@ -433,36 +509,60 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
             // a new maximum moves the reference (any number near s(m) k, so long as the sums
             // are taken against the same)
             if (mx > m) {
-                float to = mx;
-                if (CAP && way == 0) {
-                    const float q = mx * mx;
-                    float p = a.h1[BEAM_H1 - 1];
-#pragma unroll
-                    for (int i = BEAM_H1 - 2; i >= 0; i--) p = __fmaf_rn(p, q, a.h1[i]);
-                    to = mx * p;
-                } else if (CAP) {
-                    to = __fmul_rn(beam_soft<CAP>(mx, a), a.k);
+                float to = mx, f = 0.0f;
+                if constexpr (CAP == CAP_FOLD) to = beam_value<CAP>(a, mx, 0.0f);
+                if constexpr (CAP == CAP_FAR) to = beam_off(a, mx, 0.0f);
+                if (m > NEG_INF) {
+                    f = CAP == CAP_NONE ? (ref - to) * a.k : ref - to;
+                    if (CAP == CAP_FAR && !(fabsf(m) <= a.lim1 && fabsf(mx) <= a.lim1))
+                        f = beam_off(a, mx, to) - beam_off(a, m, ref) - beam_below(a, mx, m);
+                    f = ex2_approx(f);
                 }
-                const float f = m > NEG_INF ? ex2_approx(CAP ? ref - to : (ref - to) * a.k) : 0.0f;
                 s0 = mul2(s0, two(f, f));
                 s1 = mul2(s1, two(f, f));
                 m = mx;
                 ref = to;
             }
             if (way == 0) {
-                load_sum<DT, CAP ? BEAM_H1 : 0, false>(r, h1, k2, ref, s0, s1);
-            } else if (CAP && way < 3) {
+                load_sum<DT, CAP ? BEAM_H1 : 0, false, CAP == CAP_FAR>(r, h1, k2, ref, s0, s1);
+            } else if (CAP == CAP_FOLD && way < 3) {
                 uint64_t h2[BEAM_H2];
 #pragma unroll
                 for (int i = 0; i < BEAM_H2; i++) h2[i] = two(a.h2[i]);
                 if (way == 1) load_sum<DT, CAP ? BEAM_H2 : 0, false>(r, h2, k2, ref, s0, s1);
                 else load_sum<DT, CAP ? BEAM_H2 : 0, true>(r, h2, k2, ref, s0, s1);
+            } else if (CAP == CAP_FAR) {
+                float s = 0.0f;
+                const float off = beam_off(a, m, ref), none = beam_nothing(a, m);
+                uint32_t near = 0;  // the lane's vectors that hold a term
+#pragma unroll
+                for (int j = 0; j < BS_NV; j++) {
+                    float x[T::VW], most = NEG_INF;
+                    T::unpack(r[j], x);
+#pragma unroll
+                    for (int i = 0; i < T::VW; i++) most = fmaxf(most, x[i]);
+                    near |= most >= none && most > -1e30f ? 1u << j : 0u;
+                }
+                near = __reduce_or_sync(FULLMASK, near);
+                for (; near; near &= near - 1) {
+                    const int j = __ffs(near) - 1;
+#pragma unroll 4
+                    for (int i = 0; i < T::VW; i++) {
+                        // vector j's element i, of aligned rows and of others (whose lanes take every 32nd word)
+                        constexpr int WL = 4 / T::ESIZE;
+                        const int at = VEC ? (j * 32 + lane) * T::VW + i : ((j * 4 + i / WL) * 32 + lane) * WL + i % WL;
+                        const float v = at < n ? beam_raw<DT>(T::load1(p, at)) : NEG_INF;
+                        const float e = ex2_approx(off - beam_below(a, m, v));
+                        s += v == NEG_INF ? 0.0f : e;
+                    }
+                }
+                s0 = add2(s0, two(s, 0.0f));
             } else {
                 float s = 0.0f;
 #pragma unroll 4
                 for (int i = lane; i < n; i += 32) {
                     const float v = beam_raw<DT>(T::load1(p, i));
-                    const float e = ex2_approx(CAP ? __fmaf_rn(beam_soft<CAP>(v, a), a.k, -ref) : (v - ref) * a.k);
+                    const float e = ex2_approx(CAP ? __fmaf_rn(beam_soft(v, a), a.k, -ref) : (v - ref) * a.k);
                     s += v == NEG_INF ? 0.0f : e;
                 }
                 s0 = add2(s0, two(s, 0.0f));
@@ -593,7 +693,7 @@ __device__ __forceinline__ Pair pair_log(Pair s)
 
 enum { BEAM_DEAD = 0, BEAM_LIVE = 1, BEAM_DONE = 2 };
 struct BeamRow {
-    Pair base;   // score less log of the row's sum (with the softcap less ref too)
+    Pair base;   // score less log of the row's sum (with the softcap less x of its largest logit too)
     Scaled inv;  // 1 / max(length, 1)^alpha (to 2^-248: alpha 8, 2^31 tokens)
     float score, ref;
     int len, kind;
@@ -796,6 +896,13 @@ __device__ __forceinline__ uint32_t unit_mask(const char *p, int n, int lane, fl
     return m;
 }
 
+// CAP_FAR: an item's sum counts this much in the row's of maximum `top` (apart from the
+// combine, which waits for its instructions as it is).
+static __device__ __noinline__ float beam_weight(const BeamArgs &a, float top, float4 q)
+{
+    return q.z > 0.0f ? ex2_approx(-beam_below(a, top, q.x) - beam_off(a, q.x, q.y)) : 0.0f;
+}
+
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __grid_constant__ BeamArgs a)
 {
@@ -851,18 +958,28 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
         }
         const uint32_t best = __reduce_max_sync(FULLMASK, kmax);
         const bool live = kind == BEAM_LIVE && best;
+        auto full = [](uint32_t k) { return SH ? (k << SH) | (k & 0x8000u ? 0u : 0xffffu) : k; };
         if (sums) {
             BeamRow r{{0.0f, 0.0f}, {{1.0f, 0.0f}, 0}, score, 0.0f, len, kind};
             if (live) {
-                float ref = NEG_INF;
+                float f[BIPL], off = 0.0f;
+                if (a.kind == CAP_FAR) {
 #pragma unroll
-                for (int j = 0; j < BIPL; j++)
-                    if (key[j]) ref = fmaxf(ref, q[j].y);
-                r.ref = warp_max_redux(ref);
+                    for (int j = 0; j < BIPL; j++) f[j] = beam_weight(a, key2f(full(best)), q[j]);
+                } else {
+                    float ref = NEG_INF;
+#pragma unroll
+                    for (int j = 0; j < BIPL; j++)
+                        if (key[j]) ref = fmaxf(ref, q[j].y);
+                    r.ref = warp_max_redux(ref);
+                    if (a.kind == CAP_FOLD) off = beam_value<CAP_FOLD>(a, key2f(full(best)), r.ref);
+#pragma unroll
+                    for (int j = 0; j < BIPL; j++) f[j] = ex2_approx((q[j].y - r.ref) * a.ref32);
+                }
                 Pair sum{0.0f, 0.0f};
 #pragma unroll
                 for (int j = 0; j < BIPL; j++) {
-                    const Pair s = pair_sum(sum.h, key[j] ? q[j].z * ex2_approx((q[j].y - r.ref) * a.ref32) : 0.0f);
+                    const Pair s = pair_sum(sum.h, key[j] ? q[j].z * f[j] : 0.0f);
                     sum = {s.h, sum.l + s.l};
                 }
 #pragma unroll
@@ -871,9 +988,7 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
                     sum = {s.h, s.l + (sum.l + __shfl_xor_sync(FULLMASK, sum.l, d))};
                 }
                 const Pair ln = pair_log(pair_norm(sum.h, sum.l));
-                r.base = pair_add(Pair{score, 0.0f}, Pair{-ln.h, -ln.l});
-                if (a.softcap > 0.0f)  // ref is in powers of two
-                    r.base = pair_add(r.base, pair_mul(Pair{-r.ref, 0.0f}, Pair{0.693147182f, -1.904654212e-09f}));
+                r.base = pair_add(Pair{score, 0.0f}, Pair{-ln.h, __fmaf_rn(off, 0.693147182f, -ln.l)});
             }
             if (a.alpha2[0] != 0.0f)
                 r.inv = beam_length_power(max(kind == BEAM_LIVE ? len + 1 : len, 1), Pair{a.alpha2[0], a.alpha2[1]});
@@ -882,11 +997,11 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
             if (pairs) asm volatile("bar.arrive %0, 64;" ::"r"(1 + w) : "memory");
         }
         int cnt = 0;
+        Pair top{0.0f, 0.0f};  // x of the row's largest logit
         if (takes && kind == BEAM_DONE) {
             if (lane == 0) ent[w * N].y = beam_tie(w, 0u, 0u);
             cnt = 1;
         } else if (takes && live) {
-            auto full = [](uint32_t k) { return SH ? (k << SH) | (k & 0x8000u ? 0u : 0xffffu) : k; };
             int nv = 0;
 #pragma unroll
             for (int j = 0; j < BIPL; j++) nv += __popc(__ballot_sync(FULLMASK, key[j] != 0));
@@ -929,12 +1044,26 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
             }
             __syncwarp();
             const float ref = key2f(full(best));
-            for (int i = lane; i < cnt; i += 32) ent[w * N + i].x = pair_bits(beam_x(a, ref, tie_key(ent[w * N + i].y)));
+            bool have = false;
+            for (int i = lane; i < cnt; i += 32) {
+                const uint32_t k = tie_key(ent[w * N + i].y);
+                const Pair x = beam_x(a, ref, k);
+                ent[w * N + i].x = pair_bits(x);
+                if (k == full(best)) top = x, have = true;
+            }
+            const int from = __ffs(__ballot_sync(FULLMASK, have)) - 1;  // (the largest is among them)
+            top.h = __shfl_sync(FULLMASK, top.h, from);
+            top.l = __shfl_sync(FULLMASK, top.l, from);
         }
         if (takes) {
             if (pairs) asm volatile("bar.sync %0, 64;" ::"r"(1 + w) : "memory");
             else __syncwarp();
-            const BeamRow &r = s_row[w];
+            BeamRow r = s_row[w];
+            if (live && a.softcap > 0.0f) {  // the sum stands against it
+                r.base = pair_add(r.base, Pair{-top.h, -top.l});
+                __syncwarp();
+                if (lane == 0) s_row[w].base = r.base;
+            }
             uint32_t low = 0xffffffffu;
             for (int i = lane; i < cnt; i += 32) {
                 const uint64_t rank = beam_rank(r, beam_score(r, bits_pair(ent[w * N + i].x)), scaled);
@@ -1102,7 +1231,7 @@ __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __gri
     }
 }
 
-template <int DT, bool VEC, bool CAP, bool PARTS>
+template <int DT, bool VEC, int CAP, bool PARTS>
 static cudaError_t launch_stream(const BeamArgs &a, int sms, cudaStream_t s)
 {
     static int bps[MAX_DEVICES] = {};
@@ -1126,7 +1255,7 @@ static cudaError_t launch_stream(const BeamArgs &a, int sms, cudaStream_t s)
     return launch_dependent(beam_stream_kernel<DT, VEC, CAP, PARTS>, blocks < most ? blocks : most, BS_THREADS, 0, s, a);
 }
 
-template <int DT, bool VEC, bool CAP>
+template <int DT, bool VEC, int CAP>
 static cudaError_t launch_beam_t(BeamArgs &a, int sms, cudaStream_t s)
 {
     static bool ready[MAX_DEVICES] = {};
@@ -1160,11 +1289,20 @@ static cudaError_t launch_beam_t(BeamArgs &a, int sms, cudaStream_t s)
 // relative error (1.5e-8)
 static const double BEAM_TH[4] = {-0.3333314389543194, 0.13325878934833307, -0.05304549251234199, 0.017241487414783898};
 
+// Largest cap / T of CAP_FOLD and of CAP_FAR's polynomial, 256 rows of 262144 logits, cap 30:
+//   CAP_FOLD / CAP_FAR's polynomial, bf16: 41.8 / 43.5 us; scores off by at most (20 kinds of rows)
+//   at cap / T = 30 1.1e-6 / 1.6e-7, 60 2.3e-6 / 1.6e-7, 100 3.6e-6 / 1.1e-7, 400 1.6e-5 / 1.6e-7
+//   polynomial / differences: 300 44.0 / 180 us, 500 43.9 / 178; at 1000 the polynomial is off by
+//   5.7e-7, at 3000 by 3.2e-6 (43.9 / 89 us), differences by 1e-7
+constexpr double BEAM_FOLD = 64.0, BEAM_FAR = 512.0;
+
 template <int DT>
 static cudaError_t launch_beam_dt(BeamArgs &a, bool vec, int sms, cudaStream_t s)
 {
-    if (a.softcap > 0.0f) return vec ? launch_beam_t<DT, true, true>(a, sms, s) : launch_beam_t<DT, false, true>(a, sms, s);
-    return vec ? launch_beam_t<DT, true, false>(a, sms, s) : launch_beam_t<DT, false, false>(a, sms, s);
+    if (a.kind == CAP_FOLD)
+        return vec ? launch_beam_t<DT, true, CAP_FOLD>(a, sms, s) : launch_beam_t<DT, false, CAP_FOLD>(a, sms, s);
+    if (a.kind == CAP_FAR) return vec ? launch_beam_t<DT, true, CAP_FAR>(a, sms, s) : launch_beam_t<DT, false, CAP_FAR>(a, sms, s);
+    return vec ? launch_beam_t<DT, true, CAP_NONE>(a, sms, s) : launch_beam_t<DT, false, CAP_NONE>(a, sms, s);
 }
 
 cudaError_t launch_beam_select(BeamArgs &a, int dtype, bool vec, int sms, cudaStream_t s)
@@ -1182,9 +1320,14 @@ cudaError_t launch_beam_select(BeamArgs &a, int dtype, bool vec, int sms, cudaSt
     a.invcap = (float)invcap;
     // the folded coefficients stay normal numbers for caps of this range only
     const bool fold = a.softcap >= 1e-2f && a.softcap <= 1e3f;
-    a.lim1 = fold ? 0.5f * a.softcap : -1.0f;
-    a.lim2 = fold ? a.softcap : -1.0f;
-    a.skip_min = fold && (double)a.softcap * invt >= 28.0;
+    const double most = (double)a.softcap * invt;
+    a.kind = a.softcap > 0.0f ? (most <= BEAM_FOLD ? CAP_FOLD : CAP_FAR) : CAP_NONE;
+    a.lim1 = fold && most <= BEAM_FAR ? 0.5f * a.softcap : -1.0f;
+    a.lim2 = fold && a.kind == CAP_FOLD ? a.softcap : -1.0f;
+    a.skip_min = a.lim1 > 0.0f && most >= 28.0;
+    pair(2.0 * 1.4426950408889634074 * invcap, a.two2);
+    a.capk2 = (float)(2.0 * a.softcap * a.k64);
+    a.sat = 64.0f * a.softcap;
     static const double th[BEAM_H2 - 1] = {G4_TH0, G4_TH1, G4_TH2, G4_TH3, G4_TH4, G4_TH5, G4_TH6};
     a.h1[0] = a.h2[0] = a.k;
     double c = a.k64;

@@ -266,7 +266,9 @@ struct BeamArgs {
     int item_len, ipr;    // logits of an item, items a row
     int run_len, rpr;     // logits that a warp of the streaming pass takes at a time, of them a row
     int subs;             // items of such a run (1, or of one load 2, 4 or 8)
-    float k, invcap, lim1, lim2;         // lim1, lim2: largest |logit| of the two polynomials
+    int kind;                            // the softcap's (CAP_NONE, CAP_FOLD, CAP_FAR)
+    float k, invcap, lim1, lim2;         // lim1, lim2: largest |logit| of the two polynomials (-1: none)
+    float two2[2], capk2, sat;           // 2 log2(e) / cap as a pair, 2 cap k, a logit whose tanh is 1
     float ref32;                         // powers of two a unit of ref
     int skip_min;                        // whether the first polynomial may take any logit below cap / 2
     float invcap2[2], scale2[2], alpha2[2];  // 1 / cap, cap / T (or 1 / T) and alpha as pairs

@@ -441,16 +441,20 @@ typedef struct g4s_beam_state {
  * mass; a row without any other has no candidate) and +inf counts as the
  * type's largest finite number.  An ended beam has one continuation: pad_token at its
  * own score and length.  Order: score / max(length after the token,
- * 1)^length_alpha, descending, the row's sum of exponentials being off by 1e-7
- * or so; then the lower beam; within a beam the larger logit, then the lower
- * id.  Places that no continuation
- * fills get score -inf, parent and token -1, length 0, done 0.
+ * 1)^length_alpha, descending; then the lower beam; within a beam the larger
+ * logit, then the lower id.  Places that no continuation fills get score -inf,
+ * parent and token -1, length 0, done 0.
+ * Accuracy: within a beam the order is the logits'.  Between beams scores are
+ * told apart down to what a row's sum of exponentials (fp32, log-sum off by up to
+ * 4e-6) and its softcapped terms (up to 4e-7 * min(softcap / T, 64) more; 2.4e-6
+ * is the most that tests saw for softcap 30, T >= 0.5, and 4e-7 below) leave, and
+ * 3e-11 * softcap / T.  A score is returned rounded to fp32.
  *   logits        rows x row_stride elements, rows = groups * params->beams
  *   out_parents   [groups * n_out] the row continued (0..rows-1)
  *   out_tokens    [groups * n_out]
  *   in, out       out may be in (the same pointers) when n_out == beams; other
  *                 overlaps are refused.  out->lens needs in->lens.
- * softcap: 0 or below (none), or 1e-6..1e6.
+ * softcap: 0 or below (none), or 1e-6..1e6 and at most 1e8 * temperature.
  */
 int32_t g4s_beam_select(g4s_ctx *ctx, const void *logits, int32_t dtype, int32_t groups, int32_t vocab,
                         int64_t row_stride, float softcap, const g4s_beam_params *params, const g4s_beam_state *in,
