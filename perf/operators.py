@@ -409,6 +409,13 @@ def _library():
     return g4sampler, g4sampler.Sampler(device=torch.cuda.current_device(), max_rows=1024, max_vocab=262144)
 
 
+def _stream():
+    """The current stream, on which the inputs were made and the results are read.  The legacy default stream's
+    handle is 0, which the library takes for its context's own stream; 1 names it.  (By the raw handle: a Stream
+    object a call takes 3 us, as long as the smallest operator.)"""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) or 1
+
+
 def _own_select(s):
     c, o = s["case"], s["out"]
     g4, sampler = _library()
@@ -418,7 +425,8 @@ def _own_select(s):
                      g4.BeamState(o["scores"].data_ptr(), o["lens"].data_ptr(), o["done"].data_ptr()))
     params, before, after = s["plan"]
     sampler.beam_select(s["logits"].data_ptr(), g4.F32 if c["dtype"] == "f32" else g4.BF16, c["groups"], c["vocab"],
-                        s["stride"], c["softcap"], params, before, after, o["parents"].data_ptr(), o["tokens"].data_ptr())
+                        s["stride"], c["softcap"], params, before, after, o["parents"].data_ptr(), o["tokens"].data_ptr(),
+                        stream=_stream())
     return o
 
 
@@ -433,7 +441,7 @@ def _own_reorder(s):
                            H, M * D * e, c["live"] * D * e)
         hist = g4.BeamTensor(s["hist"].data_ptr(), o["hist"].data_ptr(), M * 4, 1, 0, 1, 0, c["live"] * 4)
         s["plan"] = g4.beam_tensors([kv, hist])
-    sampler.beam_reorder(s["parents"].data_ptr(), c["groups"], c["beams"], s["plan"])
+    sampler.beam_reorder(s["parents"].data_ptr(), c["groups"], c["beams"], s["plan"], stream=_stream())
     return o
 
 
@@ -453,7 +461,7 @@ def _own_fork(s):
     rows = c["groups"] * c["beams"]
     sampler.pages_fork(s["plan"], rows, s["table"].data_ptr(), s["lens"].data_ptr(), s["refs"].data_ptr(), rows,
                        s["src"].data_ptr(), c["new"], o["table"].data_ptr(), o["lens"].data_ptr(),
-                       o["refs"].data_ptr(), o["result"].data_ptr())
+                       o["refs"].data_ptr(), o["result"].data_ptr(), stream=_stream())
     return {**o, "pools": s["pools"]}
 
 
@@ -464,7 +472,7 @@ def _own_compact(s):
         s["plan"] = _cache(g4, s)
     sampler.pages_compact(s["plan"], c["seqs"], s["table"].data_ptr(), s["lens"].data_ptr(), s["refs"].data_ptr(),
                           o["table"].data_ptr(), o["refs"].data_ptr(), o["map"].data_ptr(), o["moves"].data_ptr(),
-                          o["result"].data_ptr())
+                          o["result"].data_ptr(), stream=_stream())
     return {**o, "pools": s["pools"]}
 
 
