@@ -1389,6 +1389,35 @@ static bool aliasing_ok(const void *in, const void *out, size_t in_bytes, size_t
     return a + in_bytes <= b || b + out_bytes <= a;
 }
 
+// Whether each output is memory of its own: it shares no byte with another output nor with an
+// input, except that output i may be input i itself where bit i of `same` is set.
+struct Span {
+    const void *p;  // NULL: not given
+    size_t bytes;
+};
+static bool spans_apart(std::initializer_list<Span> outs, std::initializer_list<Span> ins, unsigned same)
+{
+    int i = 0;
+    for (const Span *o = outs.begin(); o != outs.end(); o++, i++) {
+        for (const Span *q = o + 1; q != outs.end(); q++)
+            if (!aliasing_ok(o->p, q->p, o->bytes, q->bytes, false)) return false;
+        int j = 0;
+        for (const Span *q = ins.begin(); q != ins.end(); q++, j++)
+            if (!aliasing_ok(q->p, o->p, q->bytes, o->bytes, i == j && (same >> i & 1))) return false;
+    }
+    return true;
+}
+
+// Whether an array lies apart from rows of row_bytes, `stride` bytes from one to the next
+// (between two rows, for one).
+static bool apart_from_rows(Span s, const void *base, int64_t rows, int64_t row_bytes, int64_t stride)
+{
+    if (!s.p) return true;
+    const int64_t lo = (int64_t)((intptr_t)s.p - (intptr_t)base), hi = lo + (int64_t)s.bytes;
+    const int64_t first = lo < row_bytes ? 0 : (lo - row_bytes) / stride + 1;  // the first row that ends behind lo
+    return first >= rows || first * stride >= hi;
+}
+
 // Whether all arrays of 4-byte elements stand on their alignment.
 static bool aligned4(std::initializer_list<const void *> arrays)
 {
@@ -1441,9 +1470,15 @@ static int32_t beam_select_args(g4s_ctx *ctx, const char *who, const void *logit
         return fail(ctx, G4S_ERR_ARG, "%s: in->lens is NULL with a length_alpha or out->lens", who);
     const size_t ni = (size_t)groups * p->beams, no = (size_t)groups * p->n_out;
     const bool same = p->n_out == p->beams;
-    if (!aliasing_ok(in->scores, out->scores, ni * 4, no * 4, same) ||
-        !aliasing_ok(in->lens, out->lens, ni * 4, no * 4, same) || !aliasing_ok(in->done, out->done, ni, no, same))
-        return fail(ctx, G4S_ERR_ARG, "%s: out overlaps in (allowed: the same arrays, with n_out == beams)", who);
+    if (row_stride > ((int64_t)1 << 60) / (int64_t)ni)
+        return fail(ctx, G4S_ERR_ARG, "%s: row_stride %lld beyond 2^60 elements in all", who, (long long)row_stride);
+    const Span outs[5] = {{out->scores, no * 4}, {out->lens, no * 4}, {out->done, no}, {out_parents, no * 4}, {out_tokens, no * 4}};
+    bool ok = spans_apart({outs[0], outs[1], outs[2], outs[3], outs[4]},
+                          {{in->scores, ni * 4}, {in->lens, ni * 4}, {in->done, ni}}, same ? 7 : 0);
+    for (const Span &o : outs) ok = ok && apart_from_rows(o, logits, (int64_t)ni, vocab * (int64_t)esize, row_stride * (int64_t)esize);
+    if (!ok)
+        return fail(ctx, G4S_ERR_ARG,
+                    "%s: an output overlaps another, the logits or in (allowed: in's own arrays, with n_out == beams)", who);
 
     memset(&a, 0, sizeof(a));
     a.logits = logits;

@@ -452,8 +452,9 @@ typedef struct g4s_beam_state {
  *   logits        rows x row_stride elements, rows = groups * params->beams
  *   out_parents   [groups * n_out] the row continued (0..rows-1)
  *   out_tokens    [groups * n_out]
- *   in, out       out may be in (the same pointers) when n_out == beams; other
- *                 overlaps are refused.  out->lens needs in->lens.
+ *   in, out       out's arrays may be in's of the same name when n_out == beams;
+ *                 any other overlap of an output with another output, with in or
+ *                 with the logits' rows is refused.  out->lens needs in->lens.
  * softcap: 0 or below (none), or 1e-6..1e6 and at most 1e8 * temperature.
  */
 int32_t g4s_beam_select(g4s_ctx *ctx, const void *logits, int32_t dtype, int32_t groups, int32_t vocab,
