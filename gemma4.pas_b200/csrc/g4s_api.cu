@@ -1508,6 +1508,86 @@ static int32_t beam_select_args(g4s_ctx *ctx, const char *who, const void *logit
     return G4S_OK;
 }
 
+// Strided memory: count[0] x count[1] x count[2] segments of `bytes`; `extent` bytes from its
+// first to behind its last, -1 for 2^60 or more.
+struct Strided {
+    const char *p = nullptr;
+    int64_t count[3], stride[3], bytes = 0, extent = 0;
+    Strided() {}
+    Strided(const g4s_beam_tensor &t, const void *at, int64_t rows)  // a tensor's src or dst
+        : p((const char *)at), count{rows, t.segs0, t.segs1}, stride{t.row_stride, t.stride0, t.stride1}, bytes(t.seg_bytes)
+    {
+        __int128 e = bytes;
+        for (int i = 0; i < 3; i++) e += (__int128)(count[i] - 1) * stride[i];
+        extent = e < ((__int128)1 << 60) ? (int64_t)e : -1;
+    }
+};
+
+// Whether a segment of x shares a byte with one of y (of x itself: two of its segments): whether
+// whole numbers q_i, a segment's place along an axis less the other's, bring the distance
+// d + sum q_i stride_i between two segments into (-x.bytes, y.bytes).  The axes go from the
+// longest stride on, and of each only the q_i from which the shorter ones can still get there:
+// one or two, where an axis' whole extent lies within the next one's stride.  A layout that
+// takes over STEPS of them counts as overlapping.
+struct Meeting {
+    static constexpr int STEPS = 1 << 14;
+    int n = 0, steps = 0;
+    int64_t stride[6], least[6], most[6];  // axes, and the range of their q
+    int64_t low[7], high[7];               // what the axes from i on can add
+    int64_t before, behind;
+    bool self;
+
+    void add(int64_t s, int64_t from, int64_t to)
+    {
+        if (from == to) return;
+        for (int i = 0; i < n && !self; i++) {
+            if (stride[i] != s) continue;
+            least[i] += from;
+            most[i] += to;
+            return;
+        }
+        int i = n++;
+        for (; i > 0 && stride[i - 1] < s; i--) {
+            stride[i] = stride[i - 1];
+            least[i] = least[i - 1];
+            most[i] = most[i - 1];
+        }
+        stride[i] = s;
+        least[i] = from;
+        most[i] = to;
+    }
+    static int64_t floor_of(int64_t a, int64_t s) { return a / s - (a % s < 0); }
+    bool from(int i, int64_t d, bool same)
+    {
+        if (++steps > STEPS) return true;
+        if (i == n) return d > -before && d < behind && !(self && same);
+        const int64_t s = stride[i];
+        const int64_t last = std::min(most[i], -floor_of(d + low[i + 1] - behind, s) - 1);
+        for (int64_t q = std::max(least[i], floor_of(-before - high[i + 1] - d, s) + 1); q <= last; q++)
+            if (from(i + 1, d + q * s, same && q == 0)) return true;
+        return false;
+    }
+    static bool of(const Strided &x, const Strided &y)
+    {
+        const int64_t d = (int64_t)((intptr_t)x.p - (intptr_t)y.p);
+        if (d >= y.extent || -d >= x.extent) return false;
+        Meeting m;
+        m.self = &x == &y;
+        m.before = x.bytes;
+        m.behind = y.bytes;
+        for (int i = 0; i < 3; i++) m.add(x.stride[i], m.self ? 1 - x.count[i] : 0, x.count[i] - 1);
+        for (int i = 0; i < 3 && !m.self; i++) m.add(y.stride[i], 1 - y.count[i], 0);
+        m.low[m.n] = m.high[m.n] = 0;
+        bool nested = true;  // (the usual layout, without a search)
+        for (int i = m.n - 1; i >= 0; i--) {
+            nested = nested && m.stride[i] >= m.high[i + 1] + m.behind;
+            m.low[i] = m.low[i + 1] + m.least[i] * m.stride[i];
+            m.high[i] = m.high[i + 1] + m.most[i] * m.stride[i];
+        }
+        return !(m.self && nested) && m.from(0, d, true);
+    }
+};
+
 // Largest of 16, 4 and 1 that divides every value of `bits` (addresses and sizes or-ed together).
 static int copy_width(uint64_t bits) { return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1; }
 
@@ -1554,6 +1634,23 @@ static int32_t beam_reorder_args(g4s_ctx *ctx, const char *who, const int32_t *p
         a.first[a.n++] = blocks;
         blocks += (int64_t)groups * q.blocks;
         if (blocks > 0x7fffffff) return fail(ctx, G4S_ERR_CAPACITY, "%s: over 2^31 blocks of work", who);
+    }
+    Strided dst[G4S_BEAM_MAX_TENSORS], src[G4S_BEAM_MAX_TENSORS];
+    for (int i = 0; i < n_tensors; i++) {
+        const g4s_beam_tensor &t = tensors[i];
+        if (t.seg_bytes == 0) continue;
+        const bool in_place = t.src == t.dst;
+        dst[i] = Strided(t, t.dst, (int64_t)groups * beams);
+        src[i] = Strided(t, t.src, (int64_t)groups * beams);
+        if (dst[i].extent < 0) return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d]: strides beyond 2^60 bytes in all", who, i);
+        if (Meeting::of(dst[i], dst[i])) return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d]: segments or rows overlap", who, i);
+        if (!in_place && Meeting::of(dst[i], src[i]))
+            return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d]: dst overlaps src (allowed: src itself)", who, i);
+        for (int j = 0; j < i; j++) {  // (an empty tensor's extent is 0)
+            if (Meeting::of(dst[i], dst[j]) || (src[j].p != dst[j].p && Meeting::of(dst[i], src[j])) ||
+                (!in_place && Meeting::of(src[i], dst[j])))
+                return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d] and tensors[%d] overlap where one is written", who, j, i);
+        }
     }
     return G4S_OK;
 }
