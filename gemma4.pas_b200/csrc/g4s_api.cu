@@ -1636,6 +1636,7 @@ static int32_t beam_reorder_args(g4s_ctx *ctx, const char *who, const int32_t *p
         if (blocks > 0x7fffffff) return fail(ctx, G4S_ERR_CAPACITY, "%s: over 2^31 blocks of work", who);
     }
     Strided dst[G4S_BEAM_MAX_TENSORS], src[G4S_BEAM_MAX_TENSORS];
+    const Strided read(g4s_beam_tensor{nullptr, nullptr, 4, 1, 0, 1, 0, 4}, parents, (int64_t)groups * beams);
     for (int i = 0; i < n_tensors; i++) {
         const g4s_beam_tensor &t = tensors[i];
         if (t.seg_bytes == 0) continue;
@@ -1646,6 +1647,7 @@ static int32_t beam_reorder_args(g4s_ctx *ctx, const char *who, const int32_t *p
         if (Meeting::of(dst[i], dst[i])) return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d]: segments or rows overlap", who, i);
         if (!in_place && Meeting::of(dst[i], src[i]))
             return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d]: dst overlaps src (allowed: src itself)", who, i);
+        if (Meeting::of(dst[i], read)) return fail(ctx, G4S_ERR_ARG, "%s: tensors[%d]: dst overlaps the parents", who, i);
         for (int j = 0; j < i; j++) {  // (an empty tensor's extent is 0)
             if (Meeting::of(dst[i], dst[j]) || (src[j].p != dst[j].p && Meeting::of(dst[i], src[j])) ||
                 (!in_place && Meeting::of(src[i], dst[j])))
@@ -1725,6 +1727,11 @@ static int32_t pages_fork_args(g4s_ctx *ctx, const char *who, const g4s_page_cac
     if (!aliasing_ok(in->refs, out->refs, np, np, true) ||
         (n_in && n_out && !aliasing_ok(in->lens, out->lens, (size_t)n_in * 4, (size_t)n_out * 4, true)))
         return fail(ctx, G4S_ERR_ARG, "%s: out's refs or lens overlap in's (allowed: the same arrays)", who);
+    auto span = [](const void *p, size_t bytes) { return bytes ? Span{p, bytes} : Span{nullptr, 0}; };
+    const size_t no = (size_t)n_out, ni = (size_t)n_in * 4;
+    if (!spans_apart({span(out->tables, wo), span(out->lens, no * 4), {out->refs, np}, {result, 16}},
+                     {span(in->tables, wi), span(in->lens, ni), {in->refs, np}, span(src, no * 4), span(frozen, no)}, 6))
+        return fail(ctx, G4S_ERR_ARG, "%s: an array of out, or result, overlaps another array (allowed: in's lens and refs)", who);
     a.n_in = n_in;
     a.n_out = n_out;
     a.n_new = n_new;
@@ -1812,6 +1819,10 @@ int32_t g4s_pages_compact(g4s_ctx *ctx, const g4s_page_cache *cache, int32_t n_s
     const size_t w = (size_t)n_seqs * a.width * 4, np = (size_t)a.n_pages * 4;
     if ((n_seqs && !aliasing_ok(in->tables, out->tables, w, w, true)) || !aliasing_ok(in->refs, out->refs, np, np, true))
         return fail(ctx, G4S_ERR_ARG, "%s: out's tables or refs overlap in's (allowed: the same arrays)", who);
+    auto span = [](const void *p, size_t bytes) { return bytes ? Span{p, bytes} : Span{nullptr, 0}; };
+    if (!spans_apart({span(out->tables, w), {out->refs, np}, {page_map, np}, {moves, np}, {result, 16}},
+                     {span(in->tables, w), {in->refs, np}, span(in->lens, (size_t)n_seqs * 4)}, 3))
+        return fail(ctx, G4S_ERR_ARG, "%s: an output overlaps another array (allowed: in's tables and refs)", who);
     a.n_in = a.n_out = n_seqs;
     a.max_copies = a.n_pages / 2;
     a.tables_in = in->tables;
@@ -1852,6 +1863,13 @@ int32_t g4s_beam_step(g4s_ctx *ctx, const void *logits, int32_t dtype, int32_t g
     if (pages && (rc = pages_fork_args(ctx, who, pages->cache, a.rows, &pages->in, a.rows, out_parents, pages->n_new,
                                        out->done, &pages->out, pages->result, p, pools)) != G4S_OK)
         return rc;
+    if (pages) {  // the selection writes before the fork reads
+        const size_t n = (size_t)a.rows, w = n * p.width * 4, np = (size_t)p.n_pages * 4;
+        if (!spans_apart({{out->scores, n * 4}, {out->lens, n * 4}, {out->done, n}, {out_parents, n * 4}, {out_tokens, n * 4}},
+                         {{p.tables_in, w}, {p.lens_in, n * 4}, {p.refs_in, np}, {p.tables_out, w}, {p.lens_out, n * 4},
+                          {p.refs_out, np}, {p.result, 16}}, 0))
+            return fail(ctx, G4S_ERR_ARG, "%s: an output of the selection overlaps an array of the pages", who);
+    }
     DeviceGuard guard(ctx->device);
     if (!guard.ok) return fail(ctx, G4S_ERR_CUDA, "%s: cannot select device %d", who, ctx->device);
     cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;

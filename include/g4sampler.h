@@ -479,7 +479,7 @@ typedef struct g4s_beam_tensor {
 /* dst row j <- src row parents[j], for every tensor, in one launch.  A parent
    outside the row's own group (-1 among them) leaves the row as it was.
    Refused: a tensor's segments (of all rows) that overlap one another, a dst that
-   overlaps src without being it or what another tensor reads or writes, layouts
+   overlaps src without being it, parents or what another tensor reads or writes, layouts
    so entangled that this cannot be told in some 10^4 steps, and 2^60 bytes or
    more from a tensor's first byte to its last.  Fastest where all addresses,
    strides and seg_bytes are multiples of 16, then of 4. */
@@ -531,7 +531,9 @@ typedef struct g4s_page_tables {
  *           page id outside the pool -- kept, not counted).  Unless the last
  *           three are 0 no page is taken and no length grows: `out` is the fork
  *           alone.
- * out->tables is other memory than in->tables; lens and refs may be the same.
+ * out->lens and out->refs may be in's; any other overlap of out's arrays or of
+ * result with one another or with in, src or frozen is refused (pools, which
+ * must not overlap anything either, are not compared).
  * At most min(max_rows, G4S_PAGES_MAX_SEQS) sequences; tables and lens may be
  * NULL for none.
  */
@@ -541,8 +543,9 @@ int32_t g4s_pages_fork(g4s_ctx *ctx, const g4s_page_cache *cache, int32_t n_in, 
 
 /*
  * Moves the used pages (refs > 0) to the ids 0..used-1: those at or above
- * `used` go, in ascending order, to the free ids below it.  `out` may be `in`;
- * lens is only read (in->lens).
+ * `used` go, in ascending order, to the free ids below it.  out's tables and
+ * refs may be in's, other overlaps of an output are refused; lens is only read
+ * (in->lens).
  *   page_map  [n_pages] the new id of each page, -1 for a free one (for holders
  *             besides the tables)
  *   moves     [n_pages] (from, to) pairs, 8-byte aligned; only the moved ones

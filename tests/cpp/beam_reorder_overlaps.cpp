@@ -81,6 +81,13 @@ int main()
     EXPECT(({{A, B, 64, 1, 0, 1, 0, 64}, {A + 4096, B + 448, 64, 1, 0, 1, 0, 64}}), 2, 4, G4S_ERR_ARG, "where one is written");
     EXPECT(({{A, B, 64, 1, 0, 1, 0, 64}, {B, B + 4096, 64, 1, 0, 1, 0, 64}}), 2, 4, G4S_ERR_ARG, "where one is written");
     EXPECT(({{A, A, 64, 1, 0, 1, 0, 64}, {A, A, 64, 1, 0, 1, 0, 0}}), 2, 4, G4S_OK, "");  // an empty one
+    // over the parents (8 numbers at 4096), and with them between two rows
+    EXPECT(({{A, (void *)4096, 64, 1, 0, 1, 0, 64}}), 2, 4, G4S_ERR_ARG, "parents");
+    EXPECT(({{A, (void *)4124, 64, 1, 0, 1, 0, 64}}), 2, 4, G4S_ERR_ARG, "parents");
+    EXPECT(({{A, (void *)4128, 64, 1, 0, 1, 0, 64}}), 2, 4, G4S_OK, "");
+    EXPECT(({{A, (void *)4064, 64, 1, 0, 1, 0, 32}}), 2, 4, G4S_OK, "");
+    EXPECT(({{A, (void *)4064, 64, 1, 0, 1, 0, 33}}), 2, 4, G4S_ERR_ARG, "parents");
+    EXPECT(({{(void *)4096, A, 4, 1, 0, 1, 0, 4}}), 2, 4, G4S_OK, "");  // read they may be
     // beyond 2^60 bytes
     EXPECT(({{A, A, (int64_t)1 << 61, 1, 0, 1, 0, 64}}), 2, 4, G4S_ERR_ARG, "2^60");
     EXPECT(({{A, A, INT64_MAX, 1, 0, 1, 0, 64}}), 2, 4, G4S_ERR_ARG, "2^60");

@@ -8,7 +8,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "gemma4.pas_b200")
 
 
-@pytest.mark.parametrize("name", ["beam_overlaps", "beam_reorder_overlaps"])
+@pytest.mark.parametrize("name", ["beam_overlaps", "beam_reorder_overlaps", "beam_pages_overlaps"])
 def test_overlaps(tmp_path, g4, name):
     exe = str(tmp_path / name)
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
