@@ -449,7 +449,11 @@ typedef struct g4s_beam_state {
  * 4e-6) and its softcapped terms (up to 4e-7 * min(softcap / T, 64) more; 2.4e-6
  * is the most that tests saw for softcap 30, T >= 0.5, and 4e-7 below) leave, and
  * 3e-11 * softcap / T.  A score is returned rounded to fp32.
- *   logits        rows x row_stride elements, rows = groups * params->beams
+ *   logits        rows x row_stride elements, rows = groups * params->beams.
+ *                 Rows are read in pieces of 16 bytes, up to 15 bytes behind a row's
+ *                 end; where logits or row_stride are not multiples of 16 bytes, by
+ *                 whole 128-byte lines, up to 127 bytes before its start too.  These
+ *                 bytes (in the page of memory that the row's own are in) are not used
  *   out_parents   [groups * n_out] the row continued (0..rows-1)
  *   out_tokens    [groups * n_out]
  *   in, out       out's arrays may be in's of the same name when n_out == beams;
