@@ -30,9 +30,9 @@
 //
 // Measured (one B200, copy bandwidth 6570 GB/s), the whole selection: 256 bf16 rows of
 // 262144 logits, 8 beams, 16 continuations 42 us (3.2 TB/s; the streaming pass 32, without
-// its sums 23); 205 live fp32 rows 44 us (4.9 TB/s; 37, 35); 4 fp32 rows 9.2 us (5.0); 30
-// live fp32 rows of 32003 logits 9.9 us (4.2).  The streaming pass is bound by
-// instructions for bf16 rows (issue slots 58 %, the exponentials' unit 51 %, fp32 pipe
+// its sums 23); 205 live fp32 rows 45 us (4.8 TB/s; 37, 35); 4 fp32 rows 9.3 us (5.0); 30
+// live fp32 rows of 32003 logits 10.0 us (4.2).  The streaming pass is bound by
+// instructions for bf16 rows (issue slots 57 %, the exponentials' unit 51 %, fp32 pipe
 // 48 % busy at 21 warps an SM) and by memory for fp32; the combine, 4 us for 4 beams and
 // 10 for 8 beams and 16 continuations, by the latency of dependent steps: its one CTA a
 // prompt leaves most of the GPU idle, and waits for barriers and instruction fetches.
@@ -42,7 +42,8 @@
 namespace g4s {
 
 constexpr int BS_THREADS = 32;   // CTA of the streaming pass: a warp, which shares nothing with another
-constexpr int BS_CTAS = 24;      // of them on an SM: 80 registers a thread, 8 KiB a CTA
+constexpr int BS_CTAS = 24;      // of them on an SM: 80 registers a thread (the bf16 variants of
+                                 // unaligned rows spill 8 to 40 bytes, the aligned softcap one 4), 8 KiB a CTA
 constexpr int BS_STAGES = 2;     // loads a warp's ring in shared memory holds
 constexpr int BS_NV = 8;         // 16-byte vectors a lane and load (4 KiB, two units)
 constexpr int LINE = 128;        // loads of unaligned rows are copied from the line's start
@@ -619,7 +620,8 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
 // combine
 // ---------------------------------------------------------------------------
 // What is needed to more than 32 bits (the beams' scores meet here) is a sum of two fp32
-// numbers, high + low.  Measured on this GPU, one dependent 64-bit operation takes about
+// numbers, high + low: the error-free sums of Knuth (pair_sum) and Dekker (pair_norm) and the
+// product's error by a fused multiply-add (pair_mul).  Measured on this GPU, one dependent 64-bit operation takes about
 // 48 cycles and 128 scores in 64 bits 9000; the routines below are exact to 3e-11 of
 // their result (checked against 80 bits over their ranges).
 struct Pair {
@@ -903,6 +905,8 @@ static __device__ __noinline__ float beam_weight(const BeamArgs &a, float top, f
     return q.z > 0.0f ? ex2_approx(-beam_below(a, top, q.x) - beam_off(a, q.x, q.y)) : 0.0f;
 }
 
+// (64 registers at 1024 threads; the bf16 variant of unaligned rows spills 96 bytes, in its
+// units' masks.)
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(BC_THREADS, 1) beam_combine_kernel(const __grid_constant__ BeamArgs a)
 {
@@ -1346,7 +1350,10 @@ cudaError_t launch_beam_select(BeamArgs &a, int dtype, bool vec, int sms, cudaSt
 // group's rows: every row that is wanted is read before any is written, so that source
 // and destination may be the same memory without a copy or a barrier, and a parent of
 // several rows is read once.  Bound by memory: 801 MB read and written in 122 us, 6.5 TB/s,
-// the bandwidth of a copy; one prompt's 1.6 MB take 4.3 us, latency.
+// the bandwidth of a copy; one prompt's 1.6 MB take 4.3 us, latency.  With more beams the
+// columns' registers leave fewer threads on an SM to hide it (60 registers to 8 beams, 100 to
+// 16, 230 to 32): the same bytes in groups of 4, 8, 16 and 32 rows 123, 122, 130 and 150 us,
+// in place (a row that stays is not moved) 98, 115, 127 and 150.
 template <class V, int WMAX>
 __device__ __forceinline__ void reorder_column(const ReorderTensor &t, int row0, uint32_t c, const uint32_t *child)
 {
