@@ -406,14 +406,20 @@ def _library():
         sys.path.insert(0, at)
     import g4sampler
 
-    return g4sampler, g4sampler.Sampler(device=torch.cuda.current_device(), max_rows=1024, max_vocab=262144)
+    return g4sampler, g4sampler.Sampler(device=_device(), max_rows=1024, max_vocab=262144)
+
+
+@functools.lru_cache(None)
+def _device():
+    """The context's device."""
+    return torch.cuda.current_device()
 
 
 def _stream():
     """The current stream, on which the inputs were made and the results are read.  The legacy default stream's
     handle is 0, which the library takes for its context's own stream; 1 names it.  (By the raw handle: a Stream
     object a call takes 3 us, as long as the smallest operator.)"""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) or 1
+    return torch._C._cuda_getCurrentRawStream(_device()) or 1
 
 
 def _own_select(s):
