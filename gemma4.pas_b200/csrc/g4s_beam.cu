@@ -621,9 +621,9 @@ __global__ void __launch_bounds__(BS_THREADS, BS_CTAS) beam_stream_kernel(const 
 // ---------------------------------------------------------------------------
 // What is needed to more than 32 bits (the beams' scores meet here) is a sum of two fp32
 // numbers, high + low: the error-free sums of Knuth (pair_sum) and Dekker (pair_norm) and the
-// product's error by a fused multiply-add (pair_mul).  Measured on this GPU, one dependent 64-bit operation takes about
-// 48 cycles and 128 scores in 64 bits 9000; the routines below are exact to 3e-11 of
-// their result (checked against 80 bits over their ranges).
+// product's error by a fused multiply-add (pair_mul).  Measured on this GPU, one dependent
+// 64-bit operation takes about 48 cycles and 128 scores in 64 bits 9000; the routines below
+// are exact to 3e-11 of their result (checked against 80 bits over their ranges).
 struct Pair {
     float h, l;
 };
@@ -1294,8 +1294,8 @@ static cudaError_t launch_beam_t(BeamArgs &a, int sms, cudaStream_t s)
 static const double BEAM_TH[4] = {-0.3333314389543194, 0.13325878934833307, -0.05304549251234199, 0.017241487414783898};
 
 // Largest cap / T of CAP_FOLD and of CAP_FAR's polynomial, 256 rows of 262144 logits, cap 30:
-//   CAP_FOLD / CAP_FAR's polynomial, bf16: 41.8 / 43.5 us; scores off by at most (20 kinds of rows)
-//   at cap / T = 30 1.1e-6 / 1.6e-7, 60 2.3e-6 / 1.6e-7, 100 3.6e-6 / 1.1e-7, 400 1.6e-5 / 1.6e-7
+//   CAP_FOLD / CAP_FAR's polynomial, bf16: 41.8 / 43.5 us; scores off by at most (10 kinds of rows)
+//   at cap / T = 30 1.1e-6 / 1.6e-7, 60 2.3e-6 / 1.6e-7, 100 4.1e-6 / 1.1e-7, 400 2.0e-5 / 1.6e-7
 //   polynomial / differences: 300 44.0 / 180 us, 500 43.9 / 178; at 1000 the polynomial is off by
 //   5.7e-7, at 3000 by 3.2e-6 (43.9 / 89 us), differences by 1e-7
 constexpr double BEAM_FOLD = 64.0, BEAM_FAR = 512.0;

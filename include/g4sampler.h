@@ -482,11 +482,11 @@ typedef struct g4s_beam_tensor {
 
 /* dst row j <- src row parents[j], for every tensor, in one launch.  A parent
    outside the row's own group (-1 among them) leaves the row as it was.
-   Refused: a tensor's segments (of all rows) that overlap one another, a dst that
-   overlaps src without being it, parents or what another tensor reads or writes, layouts
-   so entangled that this cannot be told in some 10^4 steps, and 2^60 bytes or
-   more from a tensor's first byte to its last.  Fastest where all addresses,
-   strides and seg_bytes are multiples of 16, then of 4. */
+   Refused: a tensor's segments (of all rows) that overlap one another; a dst
+   that overlaps src without being it, parents, or what another tensor reads or
+   writes; layouts so entangled that this cannot be told in some 10^4 steps; 2^60
+   bytes or more from a tensor's first byte to its last.  Fastest where all
+   addresses, strides and seg_bytes are multiples of 16, then of 4. */
 int32_t g4s_beam_reorder(g4s_ctx *ctx, const int32_t *parents, int32_t groups, int32_t beams,
                          const g4s_beam_tensor *tensors, int32_t n_tensors, void *stream);
 
