@@ -1,4 +1,4 @@
-// Overlaps that the beam-search entry points refuse, without a GPU: the API's source built by
+// Overlaps (and ranges) that the beam selection refuses, without a GPU: the API's source built by
 // the host compiler around a context that was never created (the checks come before any CUDA
 // call).  Prints one line a failed check; exits 0 when all hold.
 #include "../../gemma4.pas_b200/csrc/g4s_api.cu"
@@ -23,6 +23,7 @@ struct Select {
     char *out[5] = {at(16384), at(20480), at(24576), at(28672), at(32768)};  // scores, lens, done, parents, tokens
     int32_t dtype = G4S_F32;
     int64_t stride = 120;
+    float cap = 30.0f;
     g4s_beam_params p;
     Select() { g4s_beam_params_defaults(&p); }
     int32_t run()
@@ -30,7 +31,7 @@ struct Select {
         BeamArgs a;
         bool vec;
         const g4s_beam_state i{(float *)in[0], (int32_t *)in[1], (uint8_t *)in[2]}, o{(float *)out[0], (int32_t *)out[1], (uint8_t *)out[2]};
-        return beam_select_args(&C, "select", logits, dtype, 2, 100, stride, 30.0f, &p, &i, &o, (int32_t *)out[3],
+        return beam_select_args(&C, "select", logits, dtype, 2, 100, stride, cap, &p, &i, &o, (int32_t *)out[3],
                                 (int32_t *)out[4], a, vec);
     }
 };
@@ -91,6 +92,12 @@ int main()
         s.out[0] = at(16384);
         EXPECT(s.run(), G4S_OK, "");
     }
+    // a softcap beyond 1e8 temperatures
+    { Select s; s.cap = 200.0f; s.p.temperature = 1e-6; EXPECT(s.run(), G4S_ERR_ARG, "temperature"); }
+    { Select s; s.cap = 1e6f; s.p.temperature = 0.0099; EXPECT(s.run(), G4S_ERR_ARG, "temperature"); }
+    { Select s; s.cap = 1e6f; s.p.temperature = 0.01; EXPECT(s.run(), G4S_OK, ""); }
+    { Select s; s.cap = 100.0f; s.p.temperature = 1e-6; EXPECT(s.run(), G4S_OK, ""); }
+    { Select s; s.cap = 0.0f; s.p.temperature = 1e-6; EXPECT(s.run(), G4S_OK, ""); }
     { Select s; s.stride = (int64_t)1 << 58; EXPECT(s.run(), G4S_ERR_ARG, "row_stride"); }
     { Select s; s.stride = (int64_t)1 << 62; EXPECT(s.run(), G4S_ERR_ARG, "row_stride"); }
     { Select s; s.stride = (int64_t)1 << 40; EXPECT(s.run(), G4S_OK, ""); }
